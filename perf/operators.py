@@ -243,9 +243,7 @@ def run(s):
     if s["op"] == "norm":
         got = runtime.rmsnorm_int8(s["x"], s["weight"], EPS, residual=s["residual"])
         # (8-bit values are returned as what they stand for)
-        values = torch.empty_like(s["x"])
-        torch.mul(got[0], got[1][:, None], out=values)
-        out = {"values": values, "scale": got[1]}
+        out = {"values": runtime.dequantize_int8(got[0], got[1]), "scale": got[1]}
         if s["residual"] is not None:
             out["residual"] = got[2]
         return out
