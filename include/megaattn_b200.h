@@ -412,6 +412,102 @@ typedef struct ma_step_args {
 
 int ma_step(ma_plan* plan, const ma_step_args* args, void* stream);
 
+/*
+ * Residual add + RMSNorm with an 8-bit result, the operand of ma_linear_quant.  Per token row over
+ * `hidden` columns:
+ *   h = bf16( float(x) + float(residual) )                     (without a residual: h = x)
+ *   y = h * rsqrt(mean(h^2) + eps) * weight in fp32,  scale = max|y| / 127,  q = round(y / scale)
+ * A row of zeros gets scale 0 and zeros; one whose sum of squares, maximum or scale is not finite gets
+ * scale NaN and zeros.  With cu_q, fa_b, fa_mb (all three or none) x is the fused launch's csym as in
+ * ma_residual_rmsnorm and `rows` counts row tiles; the other arrays are packed.  Without them x is packed
+ * too and `rows` counts rows.  Pitches are in elements: multiples of 8, q's of 16, none below hidden.
+ * x, residuals, weight and q are 16-byte aligned; hidden % 8 == 0; hidden <= 16384, rows <= 2^30 and row
+ * tiles <= 2^23 (MA_ERR_CAPACITY beyond).  residual_out may be residual_in; both are 0 without a
+ * residual.  Columns between hidden and q_pitch are left as they are.  Asynchronous on `stream`.
+ */
+typedef struct ma_rmsnorm_quant_args {
+  uint64_t x, residual_in, weight;   /* bf16                                              */
+  uint64_t residual_out;             /* bf16 [tokens, residual_out_pitch]                 */
+  uint64_t q_out;                    /* i8 [tokens, q_pitch]                              */
+  uint64_t scale_out;                /* f32 [tokens]                                      */
+  uint64_t cu_q, fa_b, fa_mb;        /* i32, or 0: packed rows                            */
+  int64_t x_pitch, residual_in_pitch, residual_out_pitch, q_pitch;
+  int32_t rows, hidden;
+  float eps;
+  int32_t reserved0;
+} ma_rmsnorm_quant_args;
+
+int ma_rmsnorm_quant(const ma_rmsnorm_quant_args* args, void* stream);
+
+/*
+ * Matrix product of 8-bit integers with a scale for each token and each output channel:
+ *   out[m, n] = (sum_k x[m, k] * weight[n, k]) * x_scale[m] * weight_scale[n]  (+ bias[n])
+ * The sum is exact (32-bit integers; inner <= 131071, MA_ERR_CAPACITY beyond), the rest is fp32 and
+ * rounded once.  x and weight: 16-byte aligned rows, pitches in elements, multiples of 16 and at least
+ * `inner`.  out_pitch >= width in elements; out_f32: fp32 output, otherwise bf16.  bias may be 0.
+ * tokens or width 0: nothing to do; inner >= 1.  Asynchronous on `stream`; no allocation.
+ * A bounded device-side wait that gives up is reported by ma_linear_status.
+ */
+typedef struct ma_linear_quant_args {
+  uint64_t x;                        /* i8 [tokens, x_pitch]                              */
+  uint64_t weight;                   /* i8 [width, weight_pitch]                          */
+  uint64_t x_scale, weight_scale;    /* f32 [tokens], [width]                             */
+  uint64_t bias;                     /* bf16 [width]                                      */
+  uint64_t out;
+  int64_t x_pitch, weight_pitch, out_pitch;
+  int32_t tokens, inner, width;
+  int32_t out_f32;
+} ma_linear_quant_args;
+
+int ma_linear_quant(const ma_linear_quant_args* args, void* stream);
+
+/*
+ * Waits for `stream` and reports whether an ma_linear_quant call on the current device gave up since the
+ * last report (MA_ERR_DEVICE_TIMEOUT, and *out says where); such a call's output is undefined.
+ */
+int ma_linear_status(void* stream, ma_status* out);
+
+/*
+ * Rows of 8-bit integers as the values they stand for: out[r, c] = q[r, c] * scale[r], rounded once to
+ * bf16 (out_f32: fp32).  q: 16-byte aligned rows, pitch a multiple of 16; out: any pitch.  Asynchronous.
+ */
+typedef struct ma_dequant_args {
+  uint64_t q, scale, out;            /* i8, f32 [rows], bf16 or f32                       */
+  int64_t q_pitch, out_pitch;
+  int32_t rows, cols, out_f32;
+  int32_t reserved0;
+} ma_dequant_args;
+
+int ma_dequant(const ma_dequant_args* args, void* stream);
+
+/*
+ * Rotary position embedding of a step's queries and new keys, with keys and values appended to a paged
+ * cache: the producer of a paged layer.  Row t belongs to sequence b, cu_q[b] <= t < cu_q[b + 1]
+ * (cu_q ascends from 0; sequences may be empty), and has position p = cache_seqlens[b] - (cu_q[b + 1] - t):
+ * the lengths count the new keys, as the paged layer's do.  q is rotated into out (which may be q
+ * itself); k, rotated, and v go to row p % 128 of page page_table[b, p / 128].  Convention and frequencies as in
+ * ma_rope_qk; angles are reduced in fp64.  Rows from cu_q[num_batch] on are left as they are.  A row whose page is
+ * not in the table or not in the cache is not appended (its q is rotated); one with p < 0 is passed
+ * over; both are counted in *dropped (may be 0).  Strides in elements, multiples of 8; q, k, v, out and
+ * caches 16-byte aligned.  Two rows with the same place in the cache leave it to either.
+ * Everything is read on the device: a captured call follows the arrays' contents.  Asynchronous on
+ * `stream`.
+ */
+typedef struct ma_rope_append_args {
+  uint64_t q, k, v;                  /* bf16 [rows, heads, 128] by the strides            */
+  uint64_t out;                      /* bf16, rotated q                                   */
+  uint64_t k_cache, v_cache;         /* bf16 [num_pages, 128, H_kv, 128]                  */
+  uint64_t cu_q;                     /* i32 [num_batch + 1]                               */
+  uint64_t cache_seqlens;            /* i32 [num_batch]                                   */
+  uint64_t page_table;               /* i32 [num_batch][table_pitch], table_width of it   */
+  uint64_t inv_freq;                 /* f32 [64]                                          */
+  uint64_t dropped;                  /* i32 [1], added to; or 0                           */
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, out_tok, out_head, table_pitch;
+  int32_t rows, num_batch, H_local, H_kv, num_pages, table_width;
+} ma_rope_append_args;
+
+int ma_rope_append(const ma_rope_append_args* args, void* stream);
+
 const char* ma_strerror(int code);
 
 #ifdef __cplusplus

@@ -29,7 +29,8 @@ MA_ERR_CAPACITY = -5
 EXPORTS = ("ma_query_device", "ma_plan_create", "ma_launch", "ma_plan_set_inputs", "ma_read_status",
            "ma_plan_destroy", "ma_strerror", "ma_fused_prefill_noalloc", "ma_residual_rmsnorm", "ma_rope_qk",
            "ma_detile", "ma_row_desc", "ma_stage_meta", "ma_plan_set_tasks", "ma_stage_tasks",
-           "ma_upload_meta", "ma_plan_set_split", "ma_step")
+           "ma_upload_meta", "ma_plan_set_split", "ma_step", "ma_rmsnorm_quant", "ma_linear_quant",
+           "ma_linear_status", "ma_rope_append", "ma_dequant")
 
 MA_NOALLOC_OSCRATCH_BYTES = 16 << 20
 MA_NOALLOC_MAX_BATCH = 512
@@ -97,6 +98,32 @@ class RopeArgs(C.Structure):
     _fields_ = [("q", C.c_uint64), ("k", C.c_uint64), ("cu_q", C.c_uint64), ("cu_k", C.c_uint64),
                 ("token_batch", C.c_uint64), ("inv_freq", C.c_uint64), ("tot_q", C.c_int32),
                 ("H_local", C.c_int32), ("H_kv", C.c_int32), ("reserved0", C.c_int32)]
+
+
+class RmsNormQuantArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint64) for n in ("x", "residual_in", "weight", "residual_out", "q_out", "scale_out",
+                                           "cu_q", "fa_b", "fa_mb")]
+                + [(n, C.c_int64) for n in ("x_pitch", "residual_in_pitch", "residual_out_pitch", "q_pitch")]
+                + [("rows", C.c_int32), ("hidden", C.c_int32), ("eps", C.c_float), ("reserved0", C.c_int32)])
+
+
+class LinearQuantArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint64) for n in ("x", "weight", "x_scale", "weight_scale", "bias", "out")]
+                + [(n, C.c_int64) for n in ("x_pitch", "weight_pitch", "out_pitch")]
+                + [(n, C.c_int32) for n in ("tokens", "inner", "width", "out_f32")])
+
+
+class DequantArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint64) for n in ("q", "scale", "out")] + [("q_pitch", C.c_int64), ("out_pitch", C.c_int64)]
+                + [(n, C.c_int32) for n in ("rows", "cols", "out_f32", "reserved0")])
+
+
+class RopeAppendArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint64) for n in ("q", "k", "v", "out", "k_cache", "v_cache", "cu_q", "cache_seqlens",
+                                           "page_table", "inv_freq", "dropped")]
+                + [(n, C.c_int64) for n in ("q_tok", "q_head", "k_tok", "k_head", "v_tok", "v_head", "out_tok",
+                                            "out_head", "table_pitch")]
+                + [(n, C.c_int32) for n in ("rows", "num_batch", "H_local", "H_kv", "num_pages", "table_width")])
 
 
 class DetileArgs(C.Structure):
@@ -168,6 +195,16 @@ def _load(path=None, audit=False):
     lib.ma_residual_rmsnorm.restype = C.c_int
     lib.ma_rope_qk.argtypes = [C.POINTER(RopeArgs), C.c_void_p]
     lib.ma_rope_qk.restype = C.c_int
+    lib.ma_rmsnorm_quant.argtypes = [C.c_void_p, C.c_void_p]
+    lib.ma_rmsnorm_quant.restype = C.c_int
+    lib.ma_linear_quant.argtypes = [C.c_void_p, C.c_void_p]
+    lib.ma_linear_quant.restype = C.c_int
+    lib.ma_linear_status.argtypes = [C.c_void_p, C.POINTER(Status)]
+    lib.ma_linear_status.restype = C.c_int
+    lib.ma_dequant.argtypes = [C.c_void_p, C.c_void_p]
+    lib.ma_dequant.restype = C.c_int
+    lib.ma_rope_append.argtypes = [C.c_void_p, C.c_void_p]
+    lib.ma_rope_append.restype = C.c_int
     lib.ma_detile.argtypes = [C.POINTER(DetileArgs), C.c_void_p]
     lib.ma_detile.restype = C.c_int
     lib.ma_row_desc.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32] + [C.c_void_p] * 5

@@ -14,8 +14,9 @@ LIB = os.path.join(HERE, "libmegaattn_b200.so")
 # (measured: +1.2 % on the attention stage).
 LIB_AUDIT = os.path.join(HERE, "libmegaattn_b200_audit.so")
 SOURCES = ["fused_prefill.cu", "cabi.cu", "noalloc.cu", "residual_rmsnorm.cu", "rope.cu",
-           "detile.cu", "meta_upload.cu", "step.cu", "meta.cpp"]
-HEADERS = ["ptx.cuh", "kparams.h", "launch.cuh", "paged.cuh", os.path.join("..", "..", "include", "megaattn_b200.h")]
+           "detile.cu", "meta_upload.cu", "step.cu", "meta.cpp", "rmsnorm_quant.cu", "linear_quant.cu", "rope_append.cu",
+           "dequant.cu"]
+HEADERS = ["ptx.cuh", "kparams.h", "launch.cuh", "paged.cuh", "append_place.h", os.path.join("..", "..", "include", "megaattn_b200.h")]
 
 
 def _stale(lib: str = None) -> bool:

@@ -23,6 +23,7 @@ int plan_encode_inputs(const ma_plan* pl, CUtensorMap* fresh, uint64_t Q, uint64
 void plan_take_inputs(ma_plan* pl, const CUtensorMap* fresh);
 void plan_inputs(const ma_plan* pl, CUtensorMap* maps);
 int plan_check_launch(const ma_plan* pl, const ma_launch_args* a);
+int encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_rows);
 }  // namespace ma
 
 struct ma_plan {
@@ -75,6 +76,20 @@ int encode(CUtensorMap* out, uint64_t base, int rank, const uint64_t* dims,
 int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace
+
+// Rows of bytes, `pitch` apart, in boxes of 128 bytes x box_rows: 128-byte swizzle, zero fill out of bounds.
+int ma::encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_t rows, uint64_t pitch,
+                        uint32_t box_rows) {
+  EncodeTiledFn enc = get_encoder();
+  if (!enc) return MA_ERR_CUDA;
+  if (base == 0 || (base & 15u) || (pitch & 15u)) return MA_ERR_INVALID;
+  const cuuint64_t dims[2] = {inner, rows}, strides[1] = {pitch};
+  const cuuint32_t box[2] = {128, box_rows}, step[2] = {1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, reinterpret_cast<void*>(base), dims, strides, box,
+                         step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MA_OK : MA_ERR_CUDA;
+}
 
 // The TMA descriptors of the path.  A 128 x 128 tile of Q, K or V is fetched by ONE
 // instruction as two 64-wide swizzled panels: the tensor is described as

@@ -6,5 +6,10 @@ from .prefill_layer import FusedPrefillLayer
 
 from .residual_rmsnorm import residual_rmsnorm
 from .rope import rope_qk_
+from .rmsnorm_int8 import residual_rmsnorm_int8, rmsnorm_int8
+from .linear_int8 import check_linear_status, dequantize_int8, linear_int8, quantize_weight_int8
+from .rope_append import rope_append
 
-__all__ = ["FusedFaOprojArWorkspace", "FusedPrefillLayer", "residual_rmsnorm", "rope_qk_"]
+__all__ = ["FusedFaOprojArWorkspace", "FusedPrefillLayer", "residual_rmsnorm", "rope_qk_", "rmsnorm_int8",
+           "residual_rmsnorm_int8", "linear_int8", "quantize_weight_int8", "dequantize_int8",
+           "check_linear_status", "rope_append"]
