@@ -114,6 +114,7 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[STAGES], s_empty[STAGES], s_done;
   __shared__ uint32_t s_tmem;
+  __shared__ float s_xs[TN];
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5;
   const uint32_t full = smem_u32(s_full), empty = smem_u32(s_empty), done = smem_u32(&s_done);
@@ -172,12 +173,22 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     }
     __syncwarp();
   }
+  // Two channels a thread in the end; their scales and the tokens' are fetched under the loads.
+  const int valid = min(TN, p.tokens - m0);
+  const int n = n0 + (tid & 63) * 2;
+  float ws[2] = {0.f, 0.f}, bias[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (n + j < p.width) {
+      ws[j] = p.w_scale[n + j];
+      if (p.bias) bias[j] = __uint_as_float(static_cast<uint32_t>(p.bias[n + j]) << 16);
+    }
+  for (int c = tid; c < valid; c += 128) s_xs[c] = p.x_scale[m0 + c];
   wait_bounded(done, 0, 0x13);
   tc_fence_after();
   __syncthreads();
 
   // Thread t holds channel t: its sums go to [token][channel] of this CTA's ring.
-  const int valid = min(TN, p.tokens - m0);
   for (int c0 = 0; c0 < valid; c0 += 16) {
     uint32_t r[16];
     tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c0, r);
@@ -191,45 +202,51 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   if (warp == 2) tmem_dealloc(tmem, kCols);
   if (splits > 1) { cluster_arrive(); cluster_wait(); }
 
-  // Two channels a thread, two tokens at a time, of this CTA's share of the tokens.
-  const int n = n0 + (tid & 63) * 2;
+  // Every CTA adds up its share of the tokens: 64 threads a token, four tokens of each half in flight.
   const int t1 = static_cast<int>(static_cast<long long>(valid) * (rank + 1) / splits);
-  float ws[2] = {0.f, 0.f}, bias[2] = {0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (n + j < p.width) {
-      ws[j] = p.w_scale[n + j];
-      if (p.bias) bias[j] = __uint_as_float(static_cast<uint32_t>(p.bias[n + j]) << 16);
-    }
   const int item = p.out_f32 ? 4 : 2;
-  const bool pair = n + 1 < p.width && (p.out_pitch & 1) == 0 &&
+  const bool both = n + 1 < p.width && (p.out_pitch & 1) == 0 &&
                     (reinterpret_cast<uint64_t>(p.out) & (2 * item - 1)) == 0;
-  for (int c = static_cast<int>(static_cast<long long>(valid) * rank / splits) + (tid >> 6); c < t1; c += 2) {
-    int2 sum = make_int2(0, 0);
-    const uint32_t at = ring + (c * 128 + (tid & 63) * 2) * 4;
+  const uint32_t mine = splits > 1 ? 0 : cluster_rank();
+  for (int c = static_cast<int>(static_cast<long long>(valid) * rank / splits) + (tid >> 6); c < t1; c += 8) {
+    int2 sum[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum[u] = make_int2(0, 0);
+#pragma unroll 2
     for (int r = 0; r < splits; ++r) {
-      const int2 v = ld_peer(peer_smem(at, splits > 1 ? r : cluster_rank()));
-      sum.x += v.x;
-      sum.y += v.y;
+      const uint32_t at = peer_smem(ring + (c * 128 + (tid & 63) * 2) * 4, mine + r);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + 2 * u < t1) {
+          const int2 v = ld_peer(at + u * 1024);
+          sum[u].x += v.x;
+          sum[u].y += v.y;
+        }
     }
-    const float xs = p.x_scale[m0 + c];
-    const float a = static_cast<float>(sum.x) * xs * ws[0] + bias[0];
-    const float b = static_cast<float>(sum.y) * xs * ws[1] + bias[1];
-    const long long o = static_cast<long long>(m0 + c) * p.out_pitch + n;
-    if (p.out_f32) {
-      float* out = static_cast<float*>(p.out) + o;
-      if (pair) *reinterpret_cast<float2*>(out) = make_float2(a, b);
-      else {
-        if (n < p.width) out[0] = a;
-        if (n + 1 < p.width) out[1] = b;
-      }
-    } else {
-      uint16_t* out = static_cast<uint16_t*>(p.out) + o;
-      const uint32_t v = pack_bf16x2(a, b);
-      if (pair) *reinterpret_cast<uint32_t*>(out) = v;
-      else {
-        if (n < p.width) out[0] = static_cast<uint16_t>(v);
-        if (n + 1 < p.width) out[1] = static_cast<uint16_t>(v >> 16);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (c + 2 * u >= t1) break;
+      const float xs = s_xs[c + 2 * u];
+      const float a = fmaf(static_cast<float>(sum[u].x) * xs, ws[0], bias[0]);
+      const float b = fmaf(static_cast<float>(sum[u].y) * xs, ws[1], bias[1]);
+      const long long o = static_cast<long long>(m0 + c + 2 * u) * p.out_pitch + n;
+      if (p.out_f32) {
+        float* out = static_cast<float*>(p.out) + o;
+        if (both) {
+          *reinterpret_cast<float2*>(out) = make_float2(a, b);
+        } else {
+          if (n < p.width) out[0] = a;
+          if (n + 1 < p.width) out[1] = b;
+        }
+      } else {
+        uint16_t* out = static_cast<uint16_t*>(p.out) + o;
+        const uint32_t v = pack_bf16x2(a, b);
+        if (both) {
+          *reinterpret_cast<uint32_t*>(out) = v;
+        } else {
+          if (n < p.width) out[0] = static_cast<uint16_t>(v);
+          if (n + 1 < p.width) out[1] = static_cast<uint16_t>(v >> 16);
+        }
       }
     }
   }
@@ -262,6 +279,270 @@ cudaError_t launch_narrow(const CUtensorMap& w, const CUtensorMap& x, const Line
   return e != cudaSuccess ? e : last;
 }
 
+// ------------------------------------------------------------------ many tokens
+// Two SMs share a tile of 256 tokens x BN channels (cta_group::2): each brings 128 token rows and half of
+// the weight rows, and one issuer runs both tensor cores, so a byte of either operand is loaded once per
+// pair.  Persistent pairs walk the tiles, 8 tiles of tokens at a time so that what runs at once shares its
+// operands in L2; the sums are double-buffered in TMEM, so the epilogue of a tile runs under the next.
+template <int BN, int STAGES>
+struct Wide {
+  static constexpr int kA = 128 * kSlab, kB = BN / 2 * kSlab, kStage = kA + kB;
+  static constexpr int kStaging = STAGES * kStage;              // 4 warps x 32 rows x 128 bytes
+  static constexpr int kCols = kStaging + 4 * 4096;             // 4 warps x BN x {scale, bias}
+  static constexpr int kSmem = kCols + 4 * BN * 8 + 1024;
+};
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the barrier at this address in both CTAs once every MMA issued so far completed.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// A load into this CTA's shared memory that is counted on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+struct WideTiles {
+  int m, n, total;
+};
+constexpr int kGroupM = 8;
+__device__ __forceinline__ void tile_at(const WideTiles& t, int i, int* m, int* n) {
+  const int per = kGroupM * t.n, g = i / per, r = i - g * per;
+  const int gm = min(kGroupM, t.m - g * kGroupM);
+  *n = r / gm;
+  *m = g * kGroupM + r - *n * gm;
+}
+
+template <int BN, int STAGES>
+__global__ void __launch_bounds__(256)
+linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                   const __grid_constant__ LinearArgs p, const WideTiles tiles) {
+  using S = Wide<BN, STAGES>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t s_full[STAGES], s_empty[STAGES], s_acc_full[2], s_acc_empty[2];
+  __shared__ uint32_t s_tmem;
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full = smem_u32(s_full), empty = smem_u32(s_empty);
+  const uint32_t acc_full = smem_u32(s_acc_full), acc_empty = smem_u32(s_acc_empty);
+  const uint32_t rank = cluster_rank();
+
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&s_tmem)), "r"(2 * BN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 8); }
+    fence_mbar_init();
+    tma_prefetch_desc(&w_map);
+    tma_prefetch_desc(&x_map);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();                          // (the other CTA's barriers are set up)
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  wait_for_previous();
+
+  const int blocks = (p.inner + kSlab - 1) / kSlab;
+  const int pair = static_cast<int>(blockIdx.x) >> 1, pairs = static_cast<int>(gridDim.x) >> 1;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t s = 0, phase = 0;
+      bool ok = true;
+      for (int i = pair; i < tiles.total && ok; i += pairs) {
+        int tm, tn;
+        tile_at(tiles, i, &tm, &tn);
+        const int m0 = tm * 256 + static_cast<int>(rank) * 128, n0 = tn * BN + static_cast<int>(rank) * (BN / 2);
+        for (int k = 0; k < blocks; ++k) {
+          ok = wait_bounded(empty + 8 * s, phase ^ 1u, 0x20);
+          if (!ok) break;
+          if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * S::kStage);
+          const uint32_t at = ring + s * S::kStage, bar = peer_smem(full + 8 * s, 0);
+          tma_load_2d_pair(at, &x_map, bar, k * kSlab, m0);
+          tma_load_2d_pair(at + S::kA, &w_map, bar, k * kSlab, n0);
+          if (++s == STAGES) { s = 0; phase ^= 1u; }
+        }
+      }
+      // every load is used, and no arrival on a barrier of this CTA outstanding, before it ends
+      for (int i = 0; i < STAGES && ok; ++i) {
+        ok = wait_bounded(empty + 8 * s, phase ^ 1u, 0x24);
+        if (++s == STAGES) { s = 0; phase ^= 1u; }
+      }
+      if (!ok) {                              // gave up: the copies in flight land long before this is over
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000u) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      uint32_t s = 0, phase = 0, it = 0;
+      bool ok = true;
+      for (int i = pair; i < tiles.total && ok; i += pairs, ++it) {
+        const uint32_t acc = it & 1u, d = tmem + acc * BN;
+        ok = wait_bounded(acc_empty + 8 * acc, ((it >> 1) & 1u) ^ 1u, 0x21);
+        tc_fence_after();
+        for (int k = 0; k < blocks && ok; ++k) {
+          ok = wait_bounded(full + 8 * s, phase, 0x22);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a = (ring + s * S::kStage) >> 4, b = a + (S::kA >> 4);
+#pragma unroll
+          for (int j = 0; j < kSlab / 32; ++j)
+            mma_i8_pair(d, smem_desc_at(kDescK, a + 2 * j), smem_desc_at(kDescK, b + 2 * j), idesc_i8(256, BN),
+                        k > 0 || j > 0);
+          tc_commit_pair(empty + 8 * s);
+          if (++s == STAGES) { s = 0; phase ^= 1u; }
+        }
+        tc_commit_pair(acc_full + 8 * acc);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int w = warp - 4;
+    const uint32_t stage = ring + S::kStaging + w * 4096;
+    const uint32_t cols = ring + S::kCols + w * BN * 8;
+    const int item = p.out_f32 ? 4 : 2;
+    const int span = 128 / item;                             // columns of a staged row
+    const bool wide = ((reinterpret_cast<uint64_t>(p.out) | static_cast<uint64_t>(p.out_pitch) * item) & 15u) == 0;
+    uint32_t it = 0;
+    for (int i = pair; i < tiles.total; i += pairs, ++it) {
+      const uint32_t acc = it & 1u;
+      int tm, tn;
+      tile_at(tiles, i, &tm, &tn);
+      const int row0 = tm * 256 + static_cast<int>(rank) * 128 + w * 32, n0 = tn * BN;
+      const float xs = row0 + lane < p.tokens ? p.x_scale[row0 + lane] : 0.f;
+#pragma unroll
+      for (int j = lane; j < BN; j += 32) {
+        const int n = n0 + j;
+        const float ws = n < p.width ? p.w_scale[n] : 0.f;
+        const float b = p.bias && n < p.width ? __uint_as_float(static_cast<uint32_t>(p.bias[n]) << 16) : 0.f;
+        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(cols + j * 8), "f"(ws), "f"(b) : "memory");
+      }
+      __syncwarp();
+      if (!wait_bounded(acc_full + 8 * acc, (it >> 1) & 1u, 0x23)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem + acc * BN + (static_cast<uint32_t>(w * 32) << 16);
+      for (int c0 = 0; c0 < BN; c0 += span) {
+        for (int h = 0; h < span; h += 32) {
+          uint32_t r[32];
+          tmem_ld32(taddr + c0 + h, r);
+          tc_wait_ld();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float w0, b0, w1, b1;
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(w0), "=f"(b0), "=f"(w1), "=f"(b1) : "r"(cols + (c0 + h + j) * 8));
+            v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])) * xs, w0, b0);
+            v[j + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + 1])) * xs, w1, b1);
+          }
+          if (p.out_f32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              st_shared_v4(stage + lane * 128 + ((j ^ (lane & 7)) << 4), __float_as_uint(v[4 * j]),
+                           __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              st_shared_v4(stage + lane * 128 + (((h / 8 + j) ^ (lane & 7)) << 4), pack_bf16x2(v[8 * j], v[8 * j + 1]),
+                           pack_bf16x2(v[8 * j + 2], v[8 * j + 3]), pack_bf16x2(v[8 * j + 4], v[8 * j + 5]),
+                           pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+          }
+        }
+        if (c0 + span >= BN) {               // all of this tile's sums are out of TMEM
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_peer(peer_smem(acc_empty + 8 * acc, 0));
+        }
+        __syncwarp();
+        const int n = n0 + c0 + (lane & 7) * (16 / item);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int row = q * 4 + (lane >> 3);
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4)));
+          if (row0 + row < p.tokens) {
+            char* o = static_cast<char*>(p.out) + (static_cast<long long>(row0 + row) * p.out_pitch + n) * item;
+            if (wide && n + 16 / item <= p.width) {
+              *reinterpret_cast<uint4*>(o) = make_uint4(x[0], x[1], x[2], x[3]);
+            } else if (p.out_f32) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (n + j < p.width) reinterpret_cast<uint32_t*>(o)[j] = x[j];
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (n + j < p.width) reinterpret_cast<uint16_t*>(o)[j] = static_cast<uint16_t>(x[j >> 1] >> (16 * (j & 1)));
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  __syncthreads();
+  tc_fence_before();
+  cluster_arrive();                          // (barriers and sums of a CTA are used by the other)
+  cluster_wait();
+  tc_fence_after();
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+}
+
+template <int BN, int STAGES>
+cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const LinearArgs& p, int sms, cudaStream_t stream) {
+  using S = Wide<BN, STAGES>;
+  auto kernel = linear_wide_kernel<BN, STAGES>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  WideTiles t;
+  t.m = (p.tokens + 255) / 256;
+  t.n = (p.width + BN - 1) / BN;
+  t.total = t.m * t.n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * (t.total < sms / 2 ? t.total : sms / 2)));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, kernel, w, x, p, t);
+  const cudaError_t last = cudaGetLastError();
+  return e != cudaSuccess ? e : last;
+}
+
 }  // namespace
 }  // namespace ma
 
@@ -287,10 +568,11 @@ extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
   p.out = reinterpret_cast<void*>(a->out);
   p.out_pitch = a->out_pitch;
   p.tokens = a->tokens; p.inner = a->inner; p.width = a->width; p.out_f32 = a->out_f32;
-  const int tn = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : p.tokens <= 128 ? 128 : 256;
-  const long long rows = (p.tokens + tn - 1) / tn;
-  if (rows > 65535) return MA_ERR_CAPACITY;
-  const long long tiles = (p.width + 127) / 128 * rows;
+  const bool wide = p.tokens > 128;
+  const int tn = wide ? 128 : p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
+  const long long rows = wide ? (p.tokens + 255) / 256 : 1;
+  if ((p.width + 127) / 128 * rows > 0x7fffffffLL / 8) return MA_ERR_CAPACITY;
+  const int tiles = (p.width + 127) / 128;
   const int blocks = (p.inner + 127) / 128;
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= 2 * sms && blocks >= splits * 4) splits *= 2;
@@ -302,12 +584,15 @@ extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
                              static_cast<uint64_t>(a->x_pitch), static_cast<uint32_t>(tn));
   if (rc != MA_OK) return rc;
   cudaError_t e;
-  switch (tn) {
-    case 16: e = ma::launch_narrow<16, 6>(w, x, p, splits, stream); break;
-    case 32: e = ma::launch_narrow<32, 5>(w, x, p, splits, stream); break;
-    case 64: e = ma::launch_narrow<64, 4>(w, x, p, splits, stream); break;
-    case 128: e = ma::launch_narrow<128, 3>(w, x, p, splits, stream); break;
-    default: e = ma::launch_narrow<256, 4>(w, x, p, splits, stream); break;
+  if (wide) {
+    e = ma::launch_wide<256, 6>(w, x, p, sms, stream);
+  } else {
+    switch (tn) {
+      case 16: e = ma::launch_narrow<16, 6>(w, x, p, splits, stream); break;
+      case 32: e = ma::launch_narrow<32, 5>(w, x, p, splits, stream); break;
+      case 64: e = ma::launch_narrow<64, 4>(w, x, p, splits, stream); break;
+      default: e = ma::launch_narrow<128, 3>(w, x, p, splits, stream); break;
+    }
   }
   return e == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
