@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/megaattn_b200.h"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -80,6 +82,11 @@ __device__ __forceinline__ int2 ld_peer(uint32_t addr) {
   return v;
 }
 
+// Brings a box to L2 only: no value is read, so it may run before what precedes the launch is complete.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
+
 struct LinearArgs {
   const float *x_scale, *w_scale;
   const uint16_t* bias;                       // (may be null)
@@ -131,7 +138,7 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  wait_for_previous();
+  let_next_start();
 
   const int rank = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int n0 = static_cast<int>(blockIdx.x) / splits * 128;
@@ -139,6 +146,9 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   const int blocks = (p.inner + kSlab - 1) / kSlab;
   const int first = static_cast<int>(static_cast<long long>(blocks) * rank / splits);
   const int count = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / splits) - first;
+  if (tid == 0)                               // the weights are on their way while the kernel before ends
+    for (int i = 0; i < min(count, STAGES); ++i) tma_prefetch_2d(&w_map, (first + i) * kSlab, n0);
+  wait_for_previous();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -253,12 +263,24 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   if (splits > 1) { cluster_arrive(); cluster_wait(); }     // (peers read this CTA's sums until here)
 }
 
+// A kernel's shared memory beyond 48 KB, allowed once per device (an attribute that outlasts the call; to
+// set it twice does no harm).
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes, int dev, std::atomic<uint64_t>* done) {
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <int TN, int STAGES>
 cudaError_t launch_narrow(const CUtensorMap& w, const CUtensorMap& x, const LinearArgs& p, int splits,
-                          cudaStream_t stream) {
+                          int dev, cudaStream_t stream) {
   using S = Narrow<TN, STAGES>;
   auto kernel = linear_narrow_kernel<TN, STAGES>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(kernel, S::kSmem, dev, &allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.width + 127) / 128 * splits), static_cast<unsigned>((p.tokens + TN - 1) / TN));
@@ -515,10 +537,12 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
 }
 
 template <int BN, int STAGES>
-cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const LinearArgs& p, int sms, cudaStream_t stream) {
+cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const LinearArgs& p, int sms, int dev,
+                        cudaStream_t stream) {
   using S = Wide<BN, STAGES>;
   auto kernel = linear_wide_kernel<BN, STAGES>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(kernel, S::kSmem, dev, &allowed);
   if (e != cudaSuccess) return e;
   WideTiles t;
   t.m = (p.tokens + 255) / 256;
@@ -585,13 +609,13 @@ extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
   if (rc != MA_OK) return rc;
   cudaError_t e;
   if (wide) {
-    e = ma::launch_wide<256, 6>(w, x, p, sms, stream);
+    e = ma::launch_wide<256, 6>(w, x, p, sms, dev, stream);
   } else {
     switch (tn) {
-      case 16: e = ma::launch_narrow<16, 6>(w, x, p, splits, stream); break;
-      case 32: e = ma::launch_narrow<32, 5>(w, x, p, splits, stream); break;
-      case 64: e = ma::launch_narrow<64, 4>(w, x, p, splits, stream); break;
-      default: e = ma::launch_narrow<128, 3>(w, x, p, splits, stream); break;
+      case 16: e = ma::launch_narrow<16, 6>(w, x, p, splits, dev, stream); break;
+      case 32: e = ma::launch_narrow<32, 5>(w, x, p, splits, dev, stream); break;
+      case 64: e = ma::launch_narrow<64, 4>(w, x, p, splits, dev, stream); break;
+      default: e = ma::launch_narrow<128, 3>(w, x, p, splits, dev, stream); break;
     }
   }
   return e == cudaSuccess ? MA_OK : MA_ERR_CUDA;

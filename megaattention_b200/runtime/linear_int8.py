@@ -18,9 +18,23 @@ import ctypes as C
 import torch
 
 from .. import _cabi
-from ._call import on_device, pitch_of, queue, rows_of
+from ._call import BF16, F32, I8, on_device, packer, pitch_of, queue
 
-_OUT = {torch.bfloat16: 0, torch.float32: 1}
+_OUT = {BF16: 0, F32: 1}
+_pack = packer(_cabi.LinearQuantArgs)
+_fn = _cabi.lib.ma_linear_quant
+_pack_dequant = packer(_cabi.DequantArgs)
+
+
+def _output(out, rows, n, dtype, dev):
+    """The output, its row pitch and whether it is fp32."""
+    if out is None:
+        assert dtype in _OUT, "bf16 or fp32"
+        return torch.empty(rows, n, dtype=dtype, device=dev), n, _OUT[dtype]
+    assert out.shape == (rows, n) and out.dtype in _OUT and out.device == dev, "out: [rows, columns] bf16 or fp32"
+    pitch, one = out.stride()
+    assert (one == 1 or n <= 1) and (pitch >= n or rows <= 1), "out: columns next to each other, no rows that overlap"
+    return out, pitch if rows > 1 else n, _OUT[out.dtype]
 
 
 def quantize_weight_int8(weight):
@@ -42,30 +56,30 @@ def linear_int8(x, x_scale, weight, weight_scale, *, bias=None, out=None, out_dt
     [out]`` fp32, ``bias [out]`` bf16 or none, all on one CUDA device; ``in`` up to 131071.  Returns
     ``[tokens, out]`` in ``out_dtype`` (bf16 or fp32), or fills ``out`` (any row pitch).  Queued on the
     current stream of that device."""
+    shape, strides, at = x.shape, x.stride(), x.data_ptr()
+    w_shape, w_strides, w_at = weight.shape, weight.stride(), weight.data_ptr()
     dev = x.device
-    assert x.is_cuda
-    rows_of(x, torch.int8, dev, 16, "x")
-    rows_of(weight, torch.int8, dev, 16, "weight")
-    tokens, inner = x.shape
-    width = weight.shape[0]
-    assert weight.shape[1] == inner and inner > 0, "x [tokens, in] and weight [out, in]"
-    for t, n, dtype in ((x_scale, tokens, torch.float32), (weight_scale, width, torch.float32),
-                        (bias, width, torch.bfloat16)):
-        if t is not None or dtype is torch.float32:
-            assert t.shape == (n,) and t.dtype == dtype and t.device == dev and t.is_contiguous()
-    if out is None:
-        out = torch.empty(tokens, width, dtype=out_dtype, device=dev)
-    else:
-        assert out.shape == (tokens, width) and out.device == dev
-        assert out.stride(1) == 1 or width <= 1
-        assert tokens <= 1 or out.stride(0) >= width, "rows of out overlap"
-    assert out.dtype in _OUT, "bf16 or fp32"
+    index = dev.index
+    assert len(shape) == 2 == len(w_shape) and shape[1] == w_shape[1] > 0, "x [tokens, in] and weight [out, in]"
+    assert x.dtype is I8 is weight.dtype and x.is_cuda and weight.get_device() == index, "int8 on one CUDA device"
+    pitch, w_pitch = pitch_of(strides, shape), pitch_of(w_strides, w_shape)
+    assert not (at | pitch | w_at | w_pitch) & 15 and (strides[1] == 1 == w_strides[1] or shape[1] == 1), \
+        "rows must start at multiples of 16 bytes, columns next to each other"
+    tokens, inner = shape
+    width = w_shape[0]
+    assert x_scale.shape == (tokens,) and x_scale.dtype is F32 and x_scale.get_device() == index and \
+        x_scale.is_contiguous(), "x_scale: [tokens] fp32"
+    assert weight_scale.shape == (width,) and weight_scale.dtype is F32 and weight_scale.get_device() == index and \
+        weight_scale.is_contiguous(), "weight_scale: [out] fp32"
+    b_at = 0
+    if bias is not None:
+        assert bias.shape == (width,) and bias.dtype is BF16 and bias.get_device() == index and bias.is_contiguous(), \
+            "bias: [out] bf16"
+        b_at = bias.data_ptr()
+    out, out_pitch, f32 = _output(out, tokens, width, out_dtype, dev)
     if tokens and width:
-        a = _cabi.LinearQuantArgs(x.data_ptr(), weight.data_ptr(), x_scale.data_ptr(), weight_scale.data_ptr(),
-                                  0 if bias is None else bias.data_ptr(), out.data_ptr(), pitch_of(x),
-                                  pitch_of(weight), out.stride(0) if tokens > 1 else width, tokens, inner, width,
-                                  _OUT[out.dtype])
-        queue(_cabi.lib.ma_linear_quant, a, dev, "ma_linear_quant")
+        queue(_fn, _pack(at, w_at, x_scale.data_ptr(), weight_scale.data_ptr(), b_at, out.data_ptr(), pitch, w_pitch,
+                         out_pitch, tokens, inner, width, f32), index, "ma_linear_quant")
     return out
 
 
@@ -74,21 +88,18 @@ def dequantize_int8(q, scale, *, out=None, out_dtype=torch.bfloat16):
     None]``, rounded once to ``out_dtype`` (bf16 or fp32): an 8-bit weight for what reads 16 bits, as
     ``FusedPrefillLayer(ws, dequantize_int8(W_o, W_o_scale).T)``, or an 8-bit activation beside it.  Queued on
     the current stream of the device."""
+    shape, strides, at = q.shape, q.stride(), q.data_ptr()
     dev = q.device
-    assert q.is_cuda
-    rows_of(q, torch.int8, dev, 16, "q")
-    rows, n = q.shape
-    assert scale.shape == (rows,) and scale.dtype == torch.float32 and scale.device == dev and scale.is_contiguous()
-    if out is None:
-        out = torch.empty(rows, n, dtype=out_dtype, device=dev)
-    else:
-        assert out.shape == (rows, n) and out.device == dev and (out.stride(1) == 1 or n <= 1)
-        assert rows <= 1 or out.stride(0) >= n, "rows of out overlap"
-    assert out.dtype in _OUT, "bf16 or fp32"
+    assert len(shape) == 2 and q.dtype is I8 and q.is_cuda, "q: [rows, n] int8 on a CUDA device"
+    pitch = pitch_of(strides, shape)
+    rows, n = shape
+    assert not (at | pitch) & 15 and (strides[1] == 1 or n <= 1), \
+        "q: rows must start at multiples of 16 bytes, columns next to each other"
+    assert scale.shape == (rows,) and scale.dtype is F32 and scale.device == dev and scale.is_contiguous()
+    out, out_pitch, f32 = _output(out, rows, n, out_dtype, dev)
     if rows and n:
-        a = _cabi.DequantArgs(q.data_ptr(), scale.data_ptr(), out.data_ptr(), pitch_of(q),
-                              out.stride(0) if rows > 1 else n, rows, n, _OUT[out.dtype], 0)
-        queue(_cabi.lib.ma_dequant, a, dev, "ma_dequant")
+        queue(_cabi.lib.ma_dequant, _pack_dequant(at, scale.data_ptr(), out.data_ptr(), pitch, out_pitch, rows, n, f32,
+                                                  0), dev.index, "ma_dequant")
     return out
 
 

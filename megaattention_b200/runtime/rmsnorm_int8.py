@@ -22,38 +22,49 @@ from __future__ import annotations
 import torch
 
 from .. import _cabi
-from ._call import pitch_of, queue, rows_of
+from ._call import BF16, F32, I8, packer, pitch_of, queue
 
-
-def _eight_bit_rows(rows, hidden, dev, out):
-    if out is None:
-        pitch = (hidden + 15) // 16 * 16
-        out = torch.empty(rows, pitch, dtype=torch.int8, device=dev)
-        return out if pitch == hidden else out[:, :hidden]
-    rows_of(out, torch.int8, dev, 16, "out")
-    assert out.shape == (rows, hidden)
-    return out
+_pack = packer(_cabi.RmsNormQuantArgs)
+_fn = _cabi.lib.ma_rmsnorm_quant
 
 
 def _queue(x, x_pitch, tokens, rows, hidden, weight, eps, residual, inplace, out, scale, dev, tiles, stream):
-    assert weight.shape == (hidden,) and weight.dtype == torch.bfloat16 and weight.device == dev
-    assert weight.is_contiguous() and weight.data_ptr() % 16 == 0
-    assert hidden % 8 == 0 and 0 < hidden <= 16384, "hidden: a multiple of 8, up to 16384"
-    q = _eight_bit_rows(tokens, hidden, dev, out)
+    at = dev.index
+    w = weight.data_ptr()
+    assert weight.shape == (hidden,) and weight.dtype is BF16 and weight.get_device() == at and \
+        weight.is_contiguous() and not w & 15, "weight: [hidden] bf16, 16-byte aligned"
+    assert not hidden & 7 and 0 < hidden <= 16384, "hidden: a multiple of 8, up to 16384"
+    if out is None:
+        q_pitch = (hidden + 15) & ~15
+        q = torch.empty(tokens, q_pitch, dtype=I8, device=dev)
+        q_at = q.data_ptr()
+        if q_pitch != hidden:
+            q = q[:, :hidden]
+    else:
+        q, q_at, strides = out, out.data_ptr(), out.stride()
+        assert q.shape == (tokens, hidden) and q.dtype is I8 and q.get_device() == at and strides[1] == 1
+        q_pitch = pitch_of(strides, q.shape)
+        assert not (q_at | q_pitch) & 15, "out: rows must start at multiples of 16 bytes"
     if scale is None:
-        scale = torch.empty(tokens, dtype=torch.float32, device=dev)
-    assert scale.shape == (tokens,) and scale.dtype == torch.float32 and scale.device == dev
-    assert scale.is_contiguous()
-    new_res, res = None, (0, 0, 0, 0)
+        scale = torch.empty(tokens, dtype=F32, device=dev)
+    else:
+        assert scale.shape == (tokens,) and scale.dtype is F32 and scale.get_device() == at and scale.is_contiguous()
+    new_res, r_in, r_out, r_pitch, n_pitch = None, 0, 0, 0, 0
     if residual is not None:
-        rows_of(residual, torch.bfloat16, dev, 16, "residual")
-        assert residual.shape == (tokens, hidden)
-        new_res = residual if inplace else torch.empty(tokens, hidden, dtype=torch.bfloat16, device=dev)
-        res = (residual.data_ptr(), new_res.data_ptr(), pitch_of(residual), pitch_of(new_res))
+        r_in, strides = residual.data_ptr(), residual.stride()
+        assert residual.shape == (tokens, hidden) and residual.dtype is BF16 and residual.get_device() == at, \
+            "residual: [tokens, hidden] bf16 on the device of x"
+        r_pitch = pitch_of(strides, residual.shape)
+        assert strides[1] == 1 and not r_in & 15 and not r_pitch & 7, \
+            "residual: rows must start at multiples of 16 bytes, columns next to each other"
+        if inplace:
+            new_res, n_pitch = residual, r_pitch
+        else:
+            new_res, n_pitch = torch.empty(tokens, hidden, dtype=BF16, device=dev), hidden
+        r_out = new_res.data_ptr()
     if tokens:
-        a = _cabi.RmsNormQuantArgs(x, res[0], weight.data_ptr(), res[1], q.data_ptr(), scale.data_ptr(), *tiles,
-                                   x_pitch, res[2], res[3], pitch_of(q), rows, hidden, eps, 0)
-        queue(_cabi.lib.ma_rmsnorm_quant, a, dev, "ma_rmsnorm_quant", stream)
+        queue(_fn, _pack(x, r_in, w, r_out, q_at, scale.data_ptr(), *tiles, x_pitch, r_pitch, n_pitch, q_pitch, rows,
+                         hidden, eps, 0), at, "ma_rmsnorm_quant", stream)
     return (q, scale) if residual is None else (q, scale, new_res)
 
 
@@ -63,12 +74,13 @@ def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, inplace: bool =
     ``(q [tokens, hidden] int8, scale [tokens] fp32)``, and the new residual stream as a third where there is a
     residual (with ``inplace`` it is updated where it is).  ``out`` and ``scale`` take the results.
     Queued on the current stream of that device."""
-    dev = x.device
-    assert x.is_cuda
-    rows_of(x, torch.bfloat16, dev, 16, "x")
+    shape, strides, at = x.shape, x.stride(), x.data_ptr()
+    assert len(shape) == 2 and x.dtype is BF16 and x.is_cuda, "x: [tokens, hidden] bf16 on a CUDA device"
+    pitch = pitch_of(strides, shape)
+    assert strides[1] == 1 and not at & 15 and not pitch & 7, \
+        "x: rows must start at multiples of 16 bytes, columns next to each other"
     assert residual is not None or not inplace, "inplace needs a residual"
-    tokens, hidden = x.shape
-    return _queue(x.data_ptr(), pitch_of(x), tokens, tokens, hidden, weight, eps, residual, inplace, out, scale, dev,
+    return _queue(at, pitch, shape[0], shape[0], shape[1], weight, eps, residual, inplace, out, scale, x.device,
                   (0, 0, 0), None)
 
 

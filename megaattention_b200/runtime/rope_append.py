@@ -20,24 +20,11 @@ from __future__ import annotations
 import torch
 
 from .. import _cabi
-from ._call import queue
+from ._call import BF16, F32, I32, packer, queue
 from .rope import default_inv_freq
 
-
-def _heads(t, dev, what):
-    assert t.dim() == 3 and t.shape[2] == 128 and t.dtype == torch.bfloat16 and t.device == dev, \
-        f"{what}: [tokens, heads, 128] bf16 on {dev}"
-    tok, head, one = t.stride()
-    assert one == 1 and t.data_ptr() % 16 == 0 and tok % 8 == 0 and head % 8 == 0 and tok >= 0 and head >= 0, \
-        f"{what}: heads must start at multiples of 16 bytes"
-    return tok, head
-
-
-def _words(t, dim, dev, what):
-    assert torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == dim and t.device == dev, \
-        f"{what}: int32 on {dev}"
-    assert t.stride(-1) == 1 or t.shape[-1] <= 1, f"{what}: columns must be next to each other"
-    return t
+_pack = packer(_cabi.RopeAppendArgs)
+_fn = _cabi.lib.ma_rope_append
 
 
 def rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, theta: float = 10000.0,
@@ -54,38 +41,53 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens
     both.  Two rows must not have the same place in the cache.  ``inv_freq [64]`` fp32 takes the place of
     ``theta``.  Queued on the current stream of the device."""
     dev = q.device
-    assert q.is_cuda
-    sq, sk, sv = _heads(q, dev, "q"), _heads(k, dev, "k"), _heads(v, dev, "v")
-    tokens, H = q.shape[:2]
-    Hkv = k.shape[1]
-    assert H and Hkv and k.shape == v.shape and k.shape[0] == tokens, "q [tokens, H, 128]; k, v [tokens, H_kv, 128]"
-    for c in (k_cache, v_cache):
-        assert c.dtype == torch.bfloat16 and c.device == dev and c.is_contiguous() and c.data_ptr() % 16 == 0
-        assert c.shape[-2:] == (Hkv, 128) and (c.dim() == 3 and c.shape[0] % 128 == 0 or
-                                               c.dim() == 4 and c.shape[1] == 128), \
-            "caches: [num_pages, 128, H_kv, 128] or [num_pages * 128, H_kv, 128]"
-    pages = k_cache.shape[0] if k_cache.dim() == 4 else k_cache.shape[0] // 128
-    assert pages and k_cache.shape == v_cache.shape
-    _words(page_table, 2, dev, "page_table")
-    _words(cache_seqlens, 1, dev, "cache_seqlens")
-    _words(cu_seqlens_q, 1, dev, "cu_seqlens_q")
+    at = dev.index
+    shape, kv, cache = q.shape, k.shape, k_cache.shape
+    tokens, H, d = shape
+    Hkv = kv[1]
+    assert d == 128 == kv[2] and kv == v.shape and kv[0] == tokens and H and Hkv, \
+        "q [tokens, H, 128]; k, v [tokens, H_kv, 128]"
+    assert q.dtype is BF16 is k.dtype and BF16 is v.dtype is k_cache.dtype and v_cache.dtype is BF16, "bf16"
+    assert q.is_cuda and k.get_device() == at == v.get_device() and k_cache.get_device() == at == v_cache.get_device(), \
+        "one CUDA device"
+    assert cache == v_cache.shape and cache[-1] == 128 and cache[-2] == Hkv and (
+        len(cache) == 4 and cache[1] == 128 or len(cache) == 3 and not cache[0] & 127) and cache[0] and \
+        k_cache.is_contiguous() and v_cache.is_contiguous(), \
+        "caches: contiguous, [num_pages, 128, H_kv, 128] or [num_pages * 128, H_kv, 128]"
+    pages = cache[0] if len(cache) == 4 else cache[0] >> 7
+    q_tok, q_head, q_one = q.stride()
+    k_tok, k_head, k_one = k.stride()
+    v_tok, v_head, v_one = v.stride()
+    q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    kc_at, vc_at = k_cache.data_ptr(), v_cache.data_ptr()
+    assert q_one == 1 == k_one == v_one and not (q_at | k_at | v_at | kc_at | vc_at) & 15 and \
+        not (q_tok | q_head | k_tok | k_head | v_tok | v_head) & 7, "heads must start at multiples of 16 bytes"
     batch, width = page_table.shape
-    assert batch and width and cache_seqlens.shape[0] == batch and cu_seqlens_q.shape[0] == batch + 1
+    assert batch and width and cache_seqlens.shape == (batch,) and cu_seqlens_q.shape == (batch + 1,), \
+        "page_table [batch, pages], cache_seqlens [batch], cu_seqlens_q [batch + 1]"
+    assert page_table.dtype is I32 is cache_seqlens.dtype and cu_seqlens_q.dtype is I32, "page_table and lengths: int32"
+    assert page_table.get_device() == at == cache_seqlens.get_device() and cu_seqlens_q.get_device() == at, \
+        "page_table and lengths: on the device of q"
+    t_pitch, t_one = page_table.stride()
+    assert (t_one == 1 or width == 1) and cache_seqlens.is_contiguous() and cu_seqlens_q.is_contiguous(), \
+        "page_table and lengths: columns next to each other"
     w = default_inv_freq(theta, dev) if inv_freq is None else inv_freq
-    assert w.shape == (64,) and w.dtype == torch.float32 and w.device == dev and w.is_contiguous()
+    assert w.shape == (64,) and w.dtype is F32 and w.get_device() == at and w.is_contiguous(), "inv_freq: [64] fp32"
     if out is None:
-        out = torch.empty(tokens, H, 128, dtype=torch.bfloat16, device=dev)
-        so = (H * 128, 128)
+        out = torch.empty(tokens, H, 128, dtype=BF16, device=dev)
+        o_at, o_tok, o_head = out.data_ptr(), H * 128, 128
     else:
-        so = _heads(out, dev, "out")
-        assert out.shape == q.shape
+        o_at = out.data_ptr()
+        o_tok, o_head, o_one = out.stride()
+        assert out.shape == shape and out.dtype is BF16 and out.get_device() == at and o_one == 1 and \
+            not o_at & 15 and not (o_tok | o_head) & 7, "out: as q"
+    d_at = 0
     if dropped is not None:
-        assert dropped.shape == (1,) and dropped.dtype == torch.int32 and dropped.device == dev
+        assert dropped.shape == (1,) and dropped.dtype is I32 and dropped.get_device() == at, "dropped: [1] int32"
+        d_at = dropped.data_ptr()
     if tokens:
-        a = _cabi.RopeAppendArgs(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            cu_seqlens_q.data_ptr(), cache_seqlens.data_ptr(), page_table.data_ptr(), w.data_ptr(),
-            0 if dropped is None else dropped.data_ptr(), *sq, *sk, *sv, *so,
-            page_table.stride(0) if batch > 1 else width, tokens, batch, H, Hkv, pages, width)
-        queue(_cabi.lib.ma_rope_append, a, dev, "ma_rope_append")
+        queue(_fn, _pack(q_at, k_at, v_at, o_at, kc_at, vc_at, cu_seqlens_q.data_ptr(), cache_seqlens.data_ptr(),
+                         page_table.data_ptr(), w.data_ptr(), d_at, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok,
+                         o_head, t_pitch if batch > 1 else width, tokens, batch, H, Hkv, pages, width), at,
+              "ma_rope_append")
     return out          # (a w made here was allocated on this stream: reuse after free is stream-ordered)
