@@ -24,6 +24,7 @@ void plan_take_inputs(ma_plan* pl, const CUtensorMap* fresh);
 void plan_inputs(const ma_plan* pl, CUtensorMap* maps);
 int plan_check_launch(const ma_plan* pl, const ma_launch_args* a);
 int encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_rows);
+int encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes);
 }  // namespace ma
 
 struct ma_plan {
@@ -88,6 +89,20 @@ int ma::encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_
   const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, reinterpret_cast<void*>(base), dims, strides, box,
                          step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MA_OK : MA_ERR_CUDA;
+}
+
+// An output's rows in boxes of 64 bytes x 32 rows, 64-byte swizzle: stores of them stop at `cols` and `rows`.
+int ma::encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes) {
+  EncodeTiledFn enc = get_encoder();
+  if (!enc) return MA_ERR_CUDA;
+  if (base == 0 || (base & 15u) || (pitch_bytes & 15u)) return MA_ERR_INVALID;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch_bytes};
+  const cuuint32_t box[2] = {f32 ? 16u : 32u, 32}, step[2] = {1, 1};
+  const CUresult r = enc(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                         reinterpret_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? MA_OK : MA_ERR_CUDA;
 }
 

@@ -13,6 +13,7 @@
 
 namespace ma {
 int encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_rows);
+int encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes);
 
 namespace {
 
@@ -309,10 +310,11 @@ cudaError_t launch_narrow(const CUtensorMap& w, const CUtensorMap& x, const Line
 template <int BN, int STAGES>
 struct Wide {
   static constexpr int kA = 128 * kSlab, kB = BN / 2 * kSlab, kStage = kA + kB;
-  static constexpr int kStaging = STAGES * kStage;              // 4 warps x 32 rows x 128 bytes
-  static constexpr int kCols = kStaging + 4 * 4096;             // 4 warps x BN x {scale, bias}
-  static constexpr int kSmem = kCols + 4 * BN * 8 + 1024;
+  static constexpr int kStaging = STAGES * kStage;              // 8 warps x 2 x 32 rows of 64 bytes
+  static constexpr int kCols = kStaging + 8 * 4096;             // 2 x {scale, bias} x BN
+  static constexpr int kSmem = kCols + 2 * 2 * BN * 4 + 1024;
 };
+constexpr int kWideThreads = 384;            // producer, issuer, TMEM, (idle), 8 warps for the epilogue
 
 __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                             uint32_t accumulate) {
@@ -340,9 +342,17 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ float4 ld_shared_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
 
 struct WideTiles {
-  int m, n, total;
+  int m, n, total, stored;                   // stored: the output takes TMA stores (16-byte rows)
 };
 constexpr int kGroupM = 8;
 __device__ __forceinline__ void tile_at(const WideTiles& t, int i, int* m, int* n) {
@@ -352,10 +362,90 @@ __device__ __forceinline__ void tile_at(const WideTiles& t, int i, int* m, int* 
   *m = g * kGroupM + r - *n * gm;
 }
 
+// 32 sums of a row to 32 outputs.
+__device__ __forceinline__ void scale_chunk(const LinearArgs& p, const uint32_t (&r)[32], float xs, uint32_t cols,
+                                            uint32_t bias_at, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 s = ld_shared_f32x4(cols + j * 4);
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.bias) b = ld_shared_f32x4(cols + bias_at + j * 4);
+    v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])) * xs, s.x, b.x);
+    v[j + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + 1])) * xs, s.y, b.y);
+    v[j + 2] = fmaf(static_cast<float>(static_cast<int>(r[j + 2])) * xs, s.z, b.z);
+    v[j + 3] = fmaf(static_cast<float>(static_cast<int>(r[j + 3])) * xs, s.w, b.w);
+  }
+}
+
+// A warp's staging: two buffers of 32 rows x 64 bytes, 16-byte pieces swizzled as the output's tensor map
+// has it (the piece's number xor bits 1-2 of the row's), in turn.
+struct Staging {
+  uint32_t base, turn;
+  // The next buffer, once the store that read it last is done with it (lane 0 issues them all).
+  __device__ __forceinline__ uint32_t next(int lane) {
+    turn ^= 1u;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+    return base + turn * 2048;
+  }
+};
+__device__ __forceinline__ void put_row(uint32_t buffer, int row, const uint32_t* u) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    st_shared_v4(buffer + row * 64 + ((j ^ ((row >> 1) & 3)) << 4), u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+}
+// 32 columns of 32 rows by TMA, which leaves out what is beyond the last row (of a row it writes 16 bytes at
+// a time, so the columns have to be there).
+__device__ __forceinline__ void store_chunk(const LinearArgs& p, const CUtensorMap* map, const float (&v)[32],
+                                            Staging* st, int n, int row0, int lane) {
+  uint32_t u[32];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    u[j] = p.out_f32 ? __float_as_uint(v[j]) : pack_bf16x2(v[2 * j], v[2 * j + 1]);
+    u[16 + j] = __float_as_uint(v[16 + j]);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h == 1 && !p.out_f32) break;
+    const uint32_t buffer = st->next(lane);
+    put_row(buffer, lane, u + 16 * h);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, buffer, n + 16 * h, row0);
+      tma_store_commit();
+    }
+  }
+}
+// The same for rows that do not start at 16 bytes and for a row's last columns: by elements, two rows at a time.
+__device__ __forceinline__ void store_elements(const LinearArgs& p, const float (&v)[32], const Staging* st, int n,
+                                               int row0, int rows, int lane) {
+  const uint32_t buffer = st->base;
+  if (lane == 0) tma_store_wait_read();      // (of every store before: the order of the buffers is left as it is)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) st_shared_f32(buffer + (lane * 16 + (j ^ (lane & 15))) * 4, v[16 * h + j]);
+    __syncwarp();
+    const int col = n + 16 * h + (lane & 15);
+    if (col >= p.width) continue;
+#pragma unroll 8
+    for (int r = lane >> 4; r < rows; r += 2) {
+      float x;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buffer + (r * 16 + ((lane & 15) ^ (r & 15))) * 4) : "memory");
+      const long long o = static_cast<long long>(row0 + r) * p.out_pitch + col;
+      if (p.out_f32) static_cast<float*>(p.out)[o] = x;
+      else static_cast<uint16_t*>(p.out)[o] = static_cast<uint16_t>(pack_bf16x2(x, 0.f));
+    }
+  }
+}
+
 template <int BN, int STAGES>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kWideThreads)
 linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
-                   const __grid_constant__ LinearArgs p, const WideTiles tiles) {
+                   const __grid_constant__ CUtensorMap out_map, const __grid_constant__ LinearArgs p,
+                   const WideTiles tiles) {
   using S = Wide<BN, STAGES>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[STAGES], s_empty[STAGES], s_acc_full[2], s_acc_empty[2];
@@ -373,10 +463,11 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 8); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 16); }
     fence_mbar_init();
     tma_prefetch_desc(&w_map);
     tma_prefetch_desc(&x_map);
+    if (tiles.stored) tma_prefetch_desc(&out_map);
   }
   tc_fence_before();
   __syncthreads();
@@ -384,10 +475,17 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
   cluster_wait();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  wait_for_previous();
+  let_next_start();
 
   const int blocks = (p.inner + kSlab - 1) / kSlab;
   const int pair = static_cast<int>(blockIdx.x) >> 1, pairs = static_cast<int>(gridDim.x) >> 1;
+  if (threadIdx.x == 0) {                    // the weights are on their way while the kernel before ends
+    int tm, tn;
+    tile_at(tiles, pair, &tm, &tn);
+    for (int k = 0; k < min(blocks, STAGES); ++k)
+      tma_prefetch_2d(&w_map, k * kSlab, tn * BN + static_cast<int>(rank) * (BN / 2));
+  }
+  wait_for_previous();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -443,89 +541,56 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int w = warp - 4;
-    const uint32_t stage = ring + S::kStaging + w * 4096;
-    const uint32_t cols = ring + S::kCols + w * BN * 8;
-    const int item = p.out_f32 ? 4 : 2;
-    const int span = 128 / item;                             // columns of a staged row
-    const bool wide = ((reinterpret_cast<uint64_t>(p.out) | static_cast<uint64_t>(p.out_pitch) * item) & 15u) == 0;
+    // Warps 4-7 take the first half of the columns, 8-11 the second; a warp reads the TMEM lanes of its
+    // number mod 4.  They meet at a barrier per tile, so a warp whose wait gave up goes through the
+    // remaining tiles without work rather than leave.
+    const int w = warp - 4, first = (w >> 2) * (BN / 2), e = threadIdx.x - 128;
+    Staging st{ring + S::kStaging + w * 4096, 0u};
     uint32_t it = 0;
+    bool ok = true;
     for (int i = pair; i < tiles.total; i += pairs, ++it) {
       const uint32_t acc = it & 1u;
       int tm, tn;
       tile_at(tiles, i, &tm, &tn);
-      const int row0 = tm * 256 + static_cast<int>(rank) * 128 + w * 32, n0 = tn * BN;
-      const float xs = row0 + lane < p.tokens ? p.x_scale[row0 + lane] : 0.f;
-#pragma unroll
-      for (int j = lane; j < BN; j += 32) {
-        const int n = n0 + j;
-        const float ws = n < p.width ? p.w_scale[n] : 0.f;
-        const float b = p.bias && n < p.width ? __uint_as_float(static_cast<uint32_t>(p.bias[n]) << 16) : 0.f;
-        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(cols + j * 8), "f"(ws), "f"(b) : "memory");
+      const int row0 = tm * 256 + static_cast<int>(rank) * 128 + (w & 3) * 32, n0 = tn * BN;
+      const int rows = min(32, p.tokens - row0);             // (none or less: beyond the last token)
+      const float xs = lane < rows ? p.x_scale[row0 + lane] : 0.f;
+      const uint32_t cols = ring + S::kCols + acc * (2 * BN * 4);
+      if (e < BN) {
+        const int n = n0 + e;
+        st_shared_f32(cols + e * 4, n < p.width ? p.w_scale[n] : 0.f);
+        if (p.bias)
+          st_shared_f32(cols + (BN + e) * 4,
+                        n < p.width ? __uint_as_float(static_cast<uint32_t>(p.bias[n]) << 16) : 0.f);
       }
-      __syncwarp();
-      if (!wait_bounded(acc_full + 8 * acc, (it >> 1) & 1u, 0x23)) break;
+      named_bar_sync(1, kWideThreads - 128);
+      if (ok) ok = wait_bounded(acc_full + 8 * acc, (it >> 1) & 1u, 0x23);
+      if (!ok) continue;
       tc_fence_after();
-      const uint32_t taddr = tmem + acc * BN + (static_cast<uint32_t>(w * 32) << 16);
-      for (int c0 = 0; c0 < BN; c0 += span) {
-        for (int h = 0; h < span; h += 32) {
-          uint32_t r[32];
-          tmem_ld32(taddr + c0 + h, r);
-          tc_wait_ld();
-          float v[32];
+      const uint32_t taddr = tmem + acc * BN + first + (static_cast<uint32_t>((w & 3) * 32) << 16);
+      uint32_t r[2][32];
+      tmem_ld32(taddr, r[0]);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float w0, b0, w1, b1;
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(w0), "=f"(b0), "=f"(w1), "=f"(b1) : "r"(cols + (c0 + h + j) * 8));
-            v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])) * xs, w0, b0);
-            v[j + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + 1])) * xs, w1, b1);
-          }
-          if (p.out_f32) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              st_shared_v4(stage + lane * 128 + ((j ^ (lane & 7)) << 4), __float_as_uint(v[4 * j]),
-                           __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              st_shared_v4(stage + lane * 128 + (((h / 8 + j) ^ (lane & 7)) << 4), pack_bf16x2(v[8 * j], v[8 * j + 1]),
-                           pack_bf16x2(v[8 * j + 2], v[8 * j + 3]), pack_bf16x2(v[8 * j + 4], v[8 * j + 5]),
-                           pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-          }
-        }
-        if (c0 + span >= BN) {               // all of this tile's sums are out of TMEM
+      for (int c = 0; c < BN / 64; ++c) {
+        tc_wait_ld();
+        if (c + 1 < BN / 64) {
+          tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+        } else {                             // all of this warp's sums are out of TMEM
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_peer(peer_smem(acc_empty + 8 * acc, 0));
         }
-        __syncwarp();
-        const int n = n0 + c0 + (lane & 7) * (16 / item);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int row = q * 4 + (lane >> 3);
-          uint32_t x[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                       : "r"(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4)));
-          if (row0 + row < p.tokens) {
-            char* o = static_cast<char*>(p.out) + (static_cast<long long>(row0 + row) * p.out_pitch + n) * item;
-            if (wide && n + 16 / item <= p.width) {
-              *reinterpret_cast<uint4*>(o) = make_uint4(x[0], x[1], x[2], x[3]);
-            } else if (p.out_f32) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (n + j < p.width) reinterpret_cast<uint32_t*>(o)[j] = x[j];
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (n + j < p.width) reinterpret_cast<uint16_t*>(o)[j] = static_cast<uint16_t>(x[j >> 1] >> (16 * (j & 1)));
-            }
-          }
+        const int n = n0 + first + c * 32;
+        if (rows > 0 && n < p.width) {       // (the same for the warp)
+          float v[32];
+          scale_chunk(p, r[c & 1], xs, cols + (first + c * 32) * 4, BN * 4, v);
+          if (tiles.stored && n + 32 <= p.width) store_chunk(p, &out_map, v, &st, n, row0, lane);
+          else store_elements(p, v, &st, n, row0, rows, lane);
         }
-        __syncwarp();
       }
     }
+    if (lane == 0) tma_store_wait_all();
+    __syncwarp();
   }
   __syncthreads();
   tc_fence_before();
@@ -537,9 +602,10 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
 }
 
 template <int BN, int STAGES>
-cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const LinearArgs& p, int sms, int dev,
-                        cudaStream_t stream) {
+cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& out, bool stored,
+                        const LinearArgs& p, int sms, int dev, cudaStream_t stream) {
   using S = Wide<BN, STAGES>;
+  static_assert(S::kSmem + 256 <= 232448, "shared memory of an SM");
   auto kernel = linear_wide_kernel<BN, STAGES>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(kernel, S::kSmem, dev, &allowed);
@@ -548,9 +614,10 @@ cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const Linear
   t.m = (p.tokens + 255) / 256;
   t.n = (p.width + BN - 1) / BN;
   t.total = t.m * t.n;
+  t.stored = stored;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * (t.total < sms / 2 ? t.total : sms / 2)));
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(kWideThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -562,7 +629,7 @@ cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const Linear
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, kernel, w, x, p, t);
+  e = cudaLaunchKernelEx(&cfg, kernel, w, x, out, p, t);
   const cudaError_t last = cudaGetLastError();
   return e != cudaSuccess ? e : last;
 }
@@ -606,10 +673,16 @@ extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
   if (rc == MA_OK)
     rc = ma::encode_bytes_2d(&x, a->x, static_cast<uint64_t>(p.inner), static_cast<uint64_t>(p.tokens),
                              static_cast<uint64_t>(a->x_pitch), static_cast<uint32_t>(tn));
+  const int item = p.out_f32 ? 4 : 2;
+  const bool stored = wide && ((a->out | static_cast<uint64_t>(p.out_pitch) * item) & 15u) == 0;
+  CUtensorMap out{};
+  if (rc == MA_OK && stored)
+    rc = ma::encode_out_2d(&out, a->out, p.out_f32 != 0, static_cast<uint64_t>(p.width),
+                           static_cast<uint64_t>(p.tokens), static_cast<uint64_t>(p.out_pitch) * item);
   if (rc != MA_OK) return rc;
   cudaError_t e;
   if (wide) {
-    e = ma::launch_wide<256, 6>(w, x, p, sms, dev, stream);
+    e = ma::launch_wide<256, 5>(w, x, out, stored, p, sms, dev, stream);
   } else {
     switch (tn) {
       case 16: e = ma::launch_narrow<16, 6>(w, x, p, splits, dev, stream); break;
