@@ -24,7 +24,8 @@ void plan_take_inputs(ma_plan* pl, const CUtensorMap* fresh);
 void plan_inputs(const ma_plan* pl, CUtensorMap* maps);
 int plan_check_launch(const ma_plan* pl, const ma_launch_args* a);
 int encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_rows);
-int encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes);
+int encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
+                  uint32_t box_bytes);
 }  // namespace ma
 
 struct ma_plan {
@@ -92,17 +93,18 @@ int ma::encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_
   return r == CUDA_SUCCESS ? MA_OK : MA_ERR_CUDA;
 }
 
-// An output's rows in boxes of 64 bytes x 32 rows, 64-byte swizzle: stores of them stop at `cols` and `rows`.
-int ma::encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes) {
+// An output's rows in boxes of box_bytes (64 or 128, swizzled as wide) x 32 rows: stores of them stop at `rows`.
+int ma::encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
+                      uint32_t box_bytes) {
   EncodeTiledFn enc = get_encoder();
   if (!enc) return MA_ERR_CUDA;
   if (base == 0 || (base & 15u) || (pitch_bytes & 15u)) return MA_ERR_INVALID;
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch_bytes};
-  const cuuint32_t box[2] = {f32 ? 16u : 32u, 32}, step[2] = {1, 1};
+  const cuuint32_t box[2] = {box_bytes / (f32 ? 4u : 2u), 32}, step[2] = {1, 1};
   const CUresult r = enc(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                          reinterpret_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? MA_OK : MA_ERR_CUDA;
 }
 

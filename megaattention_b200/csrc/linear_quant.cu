@@ -13,7 +13,8 @@
 
 namespace ma {
 int encode_bytes_2d(CUtensorMap* out, uint64_t base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_rows);
-int encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes);
+int encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
+                  uint32_t box_bytes);
 
 namespace {
 
@@ -275,14 +276,21 @@ cudaError_t allow_smem(K kernel, int bytes, int dev, std::atomic<uint64_t>* done
   return e;
 }
 
+// The tensor maps and the launch; an ma_error.
 template <int TN, int STAGES>
-cudaError_t launch_narrow(const CUtensorMap& w, const CUtensorMap& x, const LinearArgs& p, int splits,
-                          int dev, cudaStream_t stream) {
+int launch_narrow(const ma_linear_quant_args* a, const LinearArgs& p, int splits, int dev, cudaStream_t stream) {
   using S = Narrow<TN, STAGES>;
+  CUtensorMap w, x;
+  const uint64_t inner = static_cast<uint64_t>(p.inner);
+  int rc = encode_bytes_2d(&w, a->weight, inner, static_cast<uint64_t>(p.width), static_cast<uint64_t>(a->weight_pitch),
+                           128);
+  if (rc == MA_OK)
+    rc = encode_bytes_2d(&x, a->x, inner, static_cast<uint64_t>(p.tokens), static_cast<uint64_t>(a->x_pitch), TN);
+  if (rc != MA_OK) return rc;
   auto kernel = linear_narrow_kernel<TN, STAGES>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(kernel, S::kSmem, dev, &allowed);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess) return MA_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.width + 127) / 128 * splits), static_cast<unsigned>((p.tokens + TN - 1) / TN));
   cfg.blockDim = dim3(128);
@@ -299,7 +307,7 @@ cudaError_t launch_narrow(const CUtensorMap& w, const CUtensorMap& x, const Line
   cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, kernel, w, x, p, splits);
   const cudaError_t last = cudaGetLastError();
-  return e != cudaSuccess ? e : last;
+  return e == cudaSuccess && last == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
 // ------------------------------------------------------------------ many tokens
@@ -307,10 +315,11 @@ cudaError_t launch_narrow(const CUtensorMap& w, const CUtensorMap& x, const Line
 // the weight rows, and one issuer runs both tensor cores, so a byte of either operand is loaded once per
 // pair.  Persistent pairs walk the tiles, 8 tiles of tokens at a time so that what runs at once shares its
 // operands in L2; the sums are double-buffered in TMEM, so the epilogue of a tile runs under the next.
-template <int BN, int STAGES>
+template <int BN, int STAGES, bool F32>
 struct Wide {
   static constexpr int kA = 128 * kSlab, kB = BN / 2 * kSlab, kStage = kA + kB;
-  static constexpr int kStaging = STAGES * kStage;              // 8 warps x 2 x 32 rows of 64 bytes
+  static constexpr int kRow = !F32 && BN == 64 ? 64 : 128;      // bytes of a staged row
+  static constexpr int kStaging = STAGES * kStage;              // 8 warps x 32 rows
   static constexpr int kCols = kStaging + 8 * 4096;             // 2 x {scale, bias} x BN
   static constexpr int kSmem = kCols + 2 * 2 * BN * 4 + 1024;
 };
@@ -363,65 +372,40 @@ __device__ __forceinline__ void tile_at(const WideTiles& t, int i, int* m, int* 
 }
 
 // 32 sums of a row to 32 outputs.
-__device__ __forceinline__ void scale_chunk(const LinearArgs& p, const uint32_t (&r)[32], float xs, uint32_t cols,
-                                            uint32_t bias_at, float (&v)[32]) {
+__device__ __forceinline__ void scale_chunk(const uint32_t (&r)[32], float xs, uint32_t cols, uint32_t bias_at,
+                                            bool biased, float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 s = ld_shared_f32x4(cols + j * 4);
     float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.bias) b = ld_shared_f32x4(cols + bias_at + j * 4);
+    if (biased) b = ld_shared_f32x4(cols + bias_at + j * 4);
     v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])) * xs, s.x, b.x);
     v[j + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + 1])) * xs, s.y, b.y);
     v[j + 2] = fmaf(static_cast<float>(static_cast<int>(r[j + 2])) * xs, s.z, b.z);
     v[j + 3] = fmaf(static_cast<float>(static_cast<int>(r[j + 3])) * xs, s.w, b.w);
   }
 }
-
-// A warp's staging: two buffers of 32 rows x 64 bytes, 16-byte pieces swizzled as the output's tensor map
-// has it (the piece's number xor bits 1-2 of the row's), in turn.
-struct Staging {
-  uint32_t base, turn;
-  // The next buffer, once the store that read it last is done with it (lane 0 issues them all).
-  __device__ __forceinline__ uint32_t next(int lane) {
-    turn ^= 1u;
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-    __syncwarp();
-    return base + turn * 2048;
-  }
-};
-__device__ __forceinline__ void put_row(uint32_t buffer, int row, const uint32_t* u) {
+// 32 columns of this lane's row into the warp's staging: rows of ROW bytes, the columns from byte `at`, 16-byte
+// pieces swizzled as the output's tensor map has it.
+template <bool F32, int ROW>
+__device__ __forceinline__ void put_columns(const float (&v)[32], uint32_t buffer, int at, int lane) {
+  const uint32_t flip = ROW == 128 ? lane & 7 : (lane >> 1) & 3;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    st_shared_v4(buffer + row * 64 + ((j ^ ((row >> 1) & 3)) << 4), u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
-}
-// 32 columns of 32 rows by TMA, which leaves out what is beyond the last row (of a row it writes 16 bytes at
-// a time, so the columns have to be there).
-__device__ __forceinline__ void store_chunk(const LinearArgs& p, const CUtensorMap* map, const float (&v)[32],
-                                            Staging* st, int n, int row0, int lane) {
-  uint32_t u[32];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    u[j] = p.out_f32 ? __float_as_uint(v[j]) : pack_bf16x2(v[2 * j], v[2 * j + 1]);
-    u[16 + j] = __float_as_uint(v[16 + j]);
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (h == 1 && !p.out_f32) break;
-    const uint32_t buffer = st->next(lane);
-    put_row(buffer, lane, u + 16 * h);
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_2d(map, buffer, n + 16 * h, row0);
-      tma_store_commit();
-    }
+  for (int j = 0; j < (F32 ? 8 : 4); ++j) {
+    const uint32_t to = buffer + lane * ROW + (((at >> 4) + j) ^ flip) * 16;
+    if (F32)
+      st_shared_v4(to, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                   __float_as_uint(v[4 * j + 3]));
+    else
+      st_shared_v4(to, pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                   pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
   }
 }
-// The same for rows that do not start at 16 bytes and for a row's last columns: by elements, two rows at a time.
-__device__ __forceinline__ void store_elements(const LinearArgs& p, const float (&v)[32], const Staging* st, int n,
+// 32 columns of 32 rows by elements, two rows at a time: where rows do not start at 16 bytes, and a row's last
+// columns (TMA writes 16 bytes at a time, beyond the last column too).
+template <bool F32>
+__device__ __forceinline__ void store_elements(const LinearArgs& p, const float (&v)[32], uint32_t buffer, int n,
                                                int row0, int rows, int lane) {
-  const uint32_t buffer = st->base;
-  if (lane == 0) tma_store_wait_read();      // (of every store before: the order of the buffers is left as it is)
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     __syncwarp();
@@ -435,18 +419,19 @@ __device__ __forceinline__ void store_elements(const LinearArgs& p, const float 
       float x;
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buffer + (r * 16 + ((lane & 15) ^ (r & 15))) * 4) : "memory");
       const long long o = static_cast<long long>(row0 + r) * p.out_pitch + col;
-      if (p.out_f32) static_cast<float*>(p.out)[o] = x;
+      if (F32) static_cast<float*>(p.out)[o] = x;
       else static_cast<uint16_t*>(p.out)[o] = static_cast<uint16_t>(pack_bf16x2(x, 0.f));
     }
   }
+  __syncwarp();
 }
 
-template <int BN, int STAGES>
+template <int BN, int STAGES, bool F32>
 __global__ void __launch_bounds__(kWideThreads)
 linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                    const __grid_constant__ CUtensorMap out_map, const __grid_constant__ LinearArgs p,
                    const WideTiles tiles) {
-  using S = Wide<BN, STAGES>;
+  using S = Wide<BN, STAGES, F32>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[STAGES], s_empty[STAGES], s_acc_full[2], s_acc_empty[2];
   __shared__ uint32_t s_tmem;
@@ -545,7 +530,8 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     // number mod 4.  They meet at a barrier per tile, so a warp whose wait gave up goes through the
     // remaining tiles without work rather than leave.
     const int w = warp - 4, first = (w >> 2) * (BN / 2), e = threadIdx.x - 128;
-    Staging st{ring + S::kStaging + w * 4096, 0u};
+    const uint32_t staging = ring + S::kStaging + w * 4096;
+    constexpr int kItem = F32 ? 4 : 2, kChunk = S::kRow / kItem;      // columns of a staged row
     uint32_t it = 0;
     bool ok = true;
     for (int i = pair; i < tiles.total; i += pairs, ++it) {
@@ -580,12 +566,26 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
           __syncwarp();
           if (lane == 0) mbar_arrive_peer(peer_smem(acc_empty + 8 * acc, 0));
         }
-        const int n = n0 + first + c * 32;
-        if (rows > 0 && n < p.width) {       // (the same for the warp)
-          float v[32];
-          scale_chunk(p, r[c & 1], xs, cols + (first + c * 32) * 4, BN * 4, v);
-          if (tiles.stored && n + 32 <= p.width) store_chunk(p, &out_map, v, &st, n, row0, lane);
-          else store_elements(p, v, &st, n, row0, rows, lane);
+        const int n = n0 + first + c * 32, chunk = n / kChunk * kChunk;
+        if (rows <= 0 || n >= p.width) continue;                       // (the same for the warp)
+        float v[32];
+        scale_chunk(r[c & 1], xs, cols + (first + c * 32) * 4, BN * 4, p.bias != nullptr, v);
+        if (n == chunk) {                    // (the staging is free again once the store before has read it)
+          if (lane == 0) tma_store_wait_read();
+          __syncwarp();
+        }
+        if (tiles.stored && chunk + kChunk <= p.width) {
+          put_columns<F32, S::kRow>(v, staging, (n - chunk) * kItem, lane);
+          if (n + 32 == chunk + kChunk) {    // TMA leaves out rows beyond the last
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&out_map, staging, chunk, row0);
+              tma_store_commit();
+            }
+          }
+        } else {
+          store_elements<F32>(p, v, staging, n, row0, rows, lane);
         }
       }
     }
@@ -601,12 +601,12 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
 }
 
-template <int BN, int STAGES>
-cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& out, bool stored,
-                        const LinearArgs& p, int sms, int dev, cudaStream_t stream) {
-  using S = Wide<BN, STAGES>;
+template <int BN, int STAGES, bool F32>
+cudaError_t launch_wide_as(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& out, bool stored,
+                           const LinearArgs& p, int sms, int dev, cudaStream_t stream) {
+  using S = Wide<BN, STAGES, F32>;
   static_assert(S::kSmem + 256 <= 232448, "shared memory of an SM");
-  auto kernel = linear_wide_kernel<BN, STAGES>;
+  auto kernel = linear_wide_kernel<BN, STAGES, F32>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(kernel, S::kSmem, dev, &allowed);
   if (e != cudaSuccess) return e;
@@ -634,6 +634,84 @@ cudaError_t launch_wide(const CUtensorMap& w, const CUtensorMap& x, const CUtens
   return e != cudaSuccess ? e : last;
 }
 
+// The tensor maps and the launch; an ma_error.
+template <int BN, int STAGES>
+int launch_wide(const ma_linear_quant_args* a, const LinearArgs& p, int sms, int dev, cudaStream_t stream) {
+  CUtensorMap w, x, out{};
+  const uint64_t inner = static_cast<uint64_t>(p.inner), pitch = static_cast<uint64_t>(p.out_pitch) * (p.out_f32 ? 4 : 2);
+  const bool stored = ((a->out | pitch) & 15u) == 0;
+  int rc = encode_bytes_2d(&w, a->weight, inner, static_cast<uint64_t>(p.width), static_cast<uint64_t>(a->weight_pitch),
+                           BN / 2);
+  if (rc == MA_OK)
+    rc = encode_bytes_2d(&x, a->x, inner, static_cast<uint64_t>(p.tokens), static_cast<uint64_t>(a->x_pitch), 128);
+  if (rc == MA_OK && stored)
+    rc = encode_out_2d(&out, a->out, p.out_f32 != 0, static_cast<uint64_t>(p.width), static_cast<uint64_t>(p.tokens),
+                       pitch, p.out_f32 ? Wide<BN, STAGES, true>::kRow : Wide<BN, STAGES, false>::kRow);
+  if (rc != MA_OK) return rc;
+  const cudaError_t e = p.out_f32 ? launch_wide_as<BN, STAGES, true>(w, x, out, stored, p, sms, dev, stream)
+                                  : launch_wide_as<BN, STAGES, false>(w, x, out, stored, p, sms, dev, stream);
+  return e == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+}
+
+// Which kernel, and in which form, by estimates of its time in nanoseconds (device time of a call in a chain
+// of calls, beside a start and an end that all of them have):
+//   few tokens: rounds of two CTAs per SM (92 % of them: clusters leave some over) times a part's loads; what
+//   the ring holds comes at once, and parts have to be exchanged.  1 x 4096 x 10240: 3 parts 9.8 us, 2 11.8,
+//   4 15.0; 1 x 1024 x 8192: 1 part 4.2, 2 4.7; 1 x 16384 x 2304: 6 parts 10.9, 4 11.5, 1 27;
+//   many tokens: rounds of a tile per pair of SMs; 4096 x 4096 x 4096: 256 channels 48 us, 128 53, 64 89;
+//   1384 x 4096 x 1280: 15.2, 11.5, 15.9; 777 x 1000 x 1001: 12.6, 8.7, 7.2.
+// Up to 32 tokens the first always, above 512 the second; in between 64 x 4096 x 4096 takes 9.9 by the first
+// and 10.4 by the second, 256 x 4096 x 4096 12.6 and 10.8, 192 x 16384 x 2304 17.7 and 25.7.
+struct Form {
+  long long tiles, time;
+  int width, splits;                         // channels of a tile, or parts of K
+};
+Form narrow_form(const LinearArgs& p, int tn, int sms) {
+  const long long blocks = (p.inner + kSlab - 1) / kSlab;
+  const long long tiles = (p.width + 127LL) / 128 * ((p.tokens + tn - 1LL) / tn);
+  const long long room = 2LL * sms * 92 / 100;
+  Form best{0, 0, 0, 0};
+  for (int n : {1, 2, 3, 4, 6}) {
+    if (n > blocks) break;
+    const long long load = blocks * 340 / n;
+    const long long time = (tiles * n + room - 1) / room * ((load > 2040 ? load : 2040) + (n > 1 ? 1020 + 340 * n : 0));
+    if (n == 1 || time < best.time) best = {tiles * n, time, 0, n};
+  }
+  return best;
+}
+Form wide_form(const LinearArgs& p, int sms) {
+  const long long blocks = (p.inner + kSlab - 1) / kSlab;
+  constexpr int kRound[3] = {1000, 1800, 2200}, kBlock[3] = {160, 180, 290};
+  Form best{0, 0, 0, 0};
+  for (int i = 0; i < 3; ++i) {
+    const long long tiles = (p.tokens + 255LL) / 256 * ((p.width + (64LL << i) - 1) / (64LL << i));
+    const long long time = (tiles + sms / 2 - 1) / (sms / 2) * (kRound[i] + blocks * kBlock[i]);
+    if (i == 0 || time < best.time) best = {tiles, time, 64 << i, 0};
+  }
+  return best;
+}
+int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms, int dev, cudaStream_t stream) {
+  if (p.tokens <= 512) {
+    const int tn = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : 64;
+    const Form f = narrow_form(p, tn, sms);
+    if (p.tokens <= 32 || f.time <= wide_form(p, sms).time) {
+      if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
+      switch (tn) {
+        case 16: return launch_narrow<16, 6>(a, p, f.splits, dev, stream);
+        case 32: return launch_narrow<32, 5>(a, p, f.splits, dev, stream);
+        default: return launch_narrow<64, 4>(a, p, f.splits, dev, stream);
+      }
+    }
+  }
+  const Form f = wide_form(p, sms);
+  if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
+  switch (f.width) {
+    case 64: return launch_wide<64, 9>(a, p, sms, dev, stream);
+    case 128: return launch_wide<128, 7>(a, p, sms, dev, stream);
+    default: return launch_wide<256, 5>(a, p, sms, dev, stream);
+  }
+}
+
 }  // namespace
 }  // namespace ma
 
@@ -659,39 +737,7 @@ extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
   p.out = reinterpret_cast<void*>(a->out);
   p.out_pitch = a->out_pitch;
   p.tokens = a->tokens; p.inner = a->inner; p.width = a->width; p.out_f32 = a->out_f32;
-  const bool wide = p.tokens > 128;
-  const int tn = wide ? 128 : p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
-  const long long rows = wide ? (p.tokens + 255) / 256 : 1;
-  if ((p.width + 127) / 128 * rows > 0x7fffffffLL / 8) return MA_ERR_CAPACITY;
-  const int tiles = (p.width + 127) / 128;
-  const int blocks = (p.inner + 127) / 128;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * sms && blocks >= splits * 4) splits *= 2;
-  CUtensorMap w, x;
-  int rc = ma::encode_bytes_2d(&w, a->weight, static_cast<uint64_t>(p.inner), static_cast<uint64_t>(p.width),
-                               static_cast<uint64_t>(a->weight_pitch), 128);
-  if (rc == MA_OK)
-    rc = ma::encode_bytes_2d(&x, a->x, static_cast<uint64_t>(p.inner), static_cast<uint64_t>(p.tokens),
-                             static_cast<uint64_t>(a->x_pitch), static_cast<uint32_t>(tn));
-  const int item = p.out_f32 ? 4 : 2;
-  const bool stored = wide && ((a->out | static_cast<uint64_t>(p.out_pitch) * item) & 15u) == 0;
-  CUtensorMap out{};
-  if (rc == MA_OK && stored)
-    rc = ma::encode_out_2d(&out, a->out, p.out_f32 != 0, static_cast<uint64_t>(p.width),
-                           static_cast<uint64_t>(p.tokens), static_cast<uint64_t>(p.out_pitch) * item);
-  if (rc != MA_OK) return rc;
-  cudaError_t e;
-  if (wide) {
-    e = ma::launch_wide<256, 5>(w, x, out, stored, p, sms, dev, stream);
-  } else {
-    switch (tn) {
-      case 16: e = ma::launch_narrow<16, 6>(w, x, p, splits, dev, stream); break;
-      case 32: e = ma::launch_narrow<32, 5>(w, x, p, splits, dev, stream); break;
-      case 64: e = ma::launch_narrow<64, 4>(w, x, p, splits, dev, stream); break;
-      default: e = ma::launch_narrow<128, 3>(w, x, p, splits, dev, stream); break;
-    }
-  }
-  return e == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+  return ma::linear_dispatch(a, p, sms, dev, stream);
 }
 
 extern "C" int ma_linear_status(void* stream, ma_status* out) {
