@@ -1,7 +1,8 @@
 // Rows of 8-bit integers as the values they stand for: out = q * scale[row], in bf16 or fp32.
 //
-// HBM bound: 1 byte read and 2 (4) written per element.  A thread takes 16 columns, one 16-byte load and
-// two (four) 16-byte stores; rows of an output that does not start at 16 bytes are stored by elements.
+// HBM bound: 1 byte read and 2 (4) written per element.  A thread takes 16 columns of four rows at a time, one
+// 16-byte load each and 32-byte stores; rows of an output that do not start at 32 bytes are stored by 16, or
+// by elements.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -12,17 +13,32 @@ namespace ma {
 namespace {
 
 constexpr int kDqThreads = 256;
+constexpr int kDqRows = 4;                  // of a thread at a time
 
-__device__ __forceinline__ void dq_store(uint16_t* out, const float (&v)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-  *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+// 16 values to a place that is aligned to 32 bytes (wide 2) or 16.
+__device__ __forceinline__ void dq_words(char* out, const uint32_t* w, int wide) {
+  if (wide == 2) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(out), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
-__device__ __forceinline__ void dq_store(float* out, const float (&v)[8]) {
-  reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ void dq_store(uint16_t* out, const float (&v)[16], int wide) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+  dq_words(reinterpret_cast<char*>(out), w, wide);
+}
+__device__ __forceinline__ void dq_store(float* out, const float (&v)[16], int wide) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
+  dq_words(reinterpret_cast<char*>(out), w, wide);
+  dq_words(reinterpret_cast<char*>(out + 8), w + 8, wide);
 }
 __device__ __forceinline__ void dq_one(uint16_t* out, float v) {
   uint32_t w;
@@ -35,30 +51,41 @@ template <typename T>
 __global__ void __launch_bounds__(kDqThreads)
 dequant_kernel(const int8_t* q_, const float* scale_, T* out_, long long q_pitch, long long out_pitch, int rows,
                int cols, int wide) {
+  let_next_start();
   wait_for_previous();
   const int8_t* __restrict__ q = from_here(q_);
   const float* __restrict__ scale = from_here(scale_);
   T* __restrict__ out = from_here(out_);
   const int chunks = (cols + 15) / 16;
-  for (int row = blockIdx.y * blockDim.y + threadIdx.y; row < rows; row += gridDim.y * blockDim.y) {
-    const float s = scale[row];
-    for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < chunks; c += gridDim.x * blockDim.x) {
-      const uint4 v = *reinterpret_cast<const uint4*>(q + row * q_pitch + c * 16);    // (rows are 16-byte multiples)
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      T* o = out + row * out_pitch + c * 16;
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= chunks) return;
+  const int step = gridDim.y * blockDim.y;
+  for (int row = blockIdx.y * blockDim.y + threadIdx.y; row < rows; row += kDqRows * step) {
+    uint4 v[kDqRows];
+    float s[kDqRows];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float f[8];
+    for (int u = 0; u < kDqRows; ++u)
+      if (row + u * step < rows) {
+        s[u] = scale[row + u * step];
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w)
+                     : "l"(q + (row + u * step) * q_pitch + c * 16) : "memory");     // (rows are 16-byte multiples)
+      }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          f[i] = s * static_cast<float>(static_cast<int8_t>(w[2 * h + (i >> 2)] >> (8 * (i & 3))));
-        if (wide && c * 16 + 8 * h + 8 <= cols) {
-          dq_store(o + 8 * h, f);
-        } else {
+    for (int u = 0; u < kDqRows; ++u) {
+      if (row + u * step >= rows) break;
+      const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      float f[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c * 16 + 8 * h + i < cols) dq_one(o + 8 * h + i, f[i]);
-        }
+      for (int i = 0; i < 16; ++i)
+        f[i] = s[u] * static_cast<float>(static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3))));
+      T* o = out + (row + u * step) * out_pitch + c * 16;
+      if (wide && c * 16 + 16 <= cols) {
+        dq_store(o, f, wide);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c * 16 + i < cols) dq_one(o + i, f[i]);
       }
     }
   }
@@ -80,9 +107,15 @@ extern "C" int ma_dequant(const ma_dequant_args* a, void* stream) {
   const int chunks = (a->cols + 15) / 16;
   while (tx < chunks && tx < ma::kDqThreads) tx *= 2;
   const int ty = ma::kDqThreads / tx;
-  const int wide = (a->out & 15u) == 0 && (a->out_pitch * item & 15) == 0;
-  const dim3 grid(static_cast<unsigned>((chunks + tx - 1) / tx),
-                  static_cast<unsigned>((a->rows + ty - 1) / ty < 32768 ? (a->rows + ty - 1) / ty : 32768));
+  const uint64_t align = a->out | static_cast<uint64_t>(a->out_pitch) * item;
+  const int wide = (align & 31u) == 0 ? 2 : (align & 15u) == 0 ? 1 : 0;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return MA_ERR_CUDA;
+  // eight CTAs per SM, or as many as there are rows for
+  const int gx = (chunks + tx - 1) / tx, need = (a->rows + ty - 1) / ty, room = (8 * sms + gx - 1) / gx;
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(need < room ? need : room));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;

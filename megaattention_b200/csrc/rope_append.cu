@@ -56,6 +56,7 @@ __device__ __forceinline__ int sequence_of(const int* cu_q, int num_batch, int t
 }
 
 __global__ void __launch_bounds__(kRaThreads) rope_append_kernel(const __grid_constant__ RopeAppend p) {
+  let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31;
   const long long unit = static_cast<long long>(blockIdx.x) * (kRaThreads / 32) + (threadIdx.x >> 5);

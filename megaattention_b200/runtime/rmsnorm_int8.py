@@ -60,7 +60,7 @@ def _queue(x, x_pitch, tokens, rows, hidden, weight, eps, residual, inplace, out
         if inplace:
             new_res, n_pitch = residual, r_pitch
         else:
-            new_res, n_pitch = torch.empty(tokens, hidden, dtype=BF16, device=dev), hidden
+            new_res, n_pitch = torch.empty_like(residual, memory_format=torch.contiguous_format), hidden
         r_out = new_res.data_ptr()
     if tokens:
         queue(_fn, _pack(x, r_in, w, r_out, q_at, scale.data_ptr(), *tiles, x_pitch, r_pitch, n_pitch, q_pitch, rows,
