@@ -128,17 +128,17 @@ struct Row {
   }
 };
 
-// CTAs of T threads (32: of 256, a row to each warp), as many as registers allow: 64 a thread with two chunks
-// and a residual, 85 with four and none, 128 with eight.
+// CTAs of T threads (32: of 256, a row to each warp), as many as registers allow: 85 a thread with four
+// chunks and no residual, 128 with a residual or eight chunks; 64 KB are on their way to an SM then.
 constexpr int threads_of(int T) { return T == 32 ? 256 : T; }
-constexpr int ctas_of(int NCH, int T) { return (NCH > 4 ? 512 : NCH > 2 ? 768 : 1024) / threads_of(T); }
+constexpr int ctas_of(int NCH, int T, bool RES) { return (NCH > 4 || (RES && NCH > 2) ? 512 : NCH > 2 ? 768 : 1024) / threads_of(T); }
 
 // T threads on a row, NCH chunks of 8 columns each; the next row is on its way while a row is worked on.
 // Without a residual there is half as much to load and the instructions count: 15.8 of them per element
 // kept 73 % of the issue slots busy at 4.5 TB/s.  What a row costs beside its columns is spread over four
 // chunks a thread then, the weights lie in shared memory as fp32, and pitches are 32 bits.
 template <int NCH, int T, bool RES>
-__global__ void __launch_bounds__(threads_of(T), ctas_of(NCH, T))
+__global__ void __launch_bounds__(threads_of(T), ctas_of(NCH, T, RES))
 rmsnorm_quant_kernel(const __grid_constant__ NormQuant p) {
   constexpr int kWarps = T / 32, kPad = kWarps < 4 ? 4 : kWarps;
   __shared__ __align__(16) float s_sum[2][kPad], s_top[2][kPad];
@@ -245,7 +245,7 @@ rmsnorm_quant_kernel(const __grid_constant__ NormQuant p) {
 template <int NCH, int T, bool RES>
 cudaError_t launch_norm_quant(const NormQuant& p, int sms, cudaStream_t stream) {
   constexpr int threads = threads_of(T);
-  const int ctas = (p.slots + threads / T - 1) / (threads / T), room = sms * ctas_of(NCH, T);
+  const int ctas = (p.slots + threads / T - 1) / (threads / T), room = sms * ctas_of(NCH, T, RES);
   return launch_behind(rmsnorm_quant_kernel<NCH, T, RES>, ctas < room ? ctas : room, threads, 0, stream, p);
 }
 
@@ -296,11 +296,11 @@ extern "C" int ma_rmsnorm_quant(const ma_rmsnorm_quant_args* a, void* stream) {
   cudaError_t e;
   if (a->residual_in) {
     if (chunks <= 64) e = ma::launch_norm_quant<2, 32, true>(p, sms, st);
-    else if (chunks <= 128) e = ma::launch_norm_quant<2, 64, true>(p, sms, st);
-    else if (chunks <= 256) e = ma::launch_norm_quant<2, 128, true>(p, sms, st);
-    else if (chunks <= 512) e = ma::launch_norm_quant<2, 256, true>(p, sms, st);
-    else if (chunks <= 1024) e = ma::launch_norm_quant<2, 512, true>(p, sms, st);
-    else e = ma::launch_norm_quant<2, 1024, true>(p, sms, st);
+    else if (chunks <= 128) e = ma::launch_norm_quant<4, 32, true>(p, sms, st);
+    else if (chunks <= 256) e = ma::launch_norm_quant<4, 64, true>(p, sms, st);
+    else if (chunks <= 512) e = ma::launch_norm_quant<4, 128, true>(p, sms, st);
+    else if (chunks <= 1024) e = ma::launch_norm_quant<4, 256, true>(p, sms, st);
+    else e = ma::launch_norm_quant<4, 512, true>(p, sms, st);
   } else {
     if (chunks <= 64) e = ma::launch_norm_quant<2, 32, false>(p, sms, st);
     else if (chunks <= 128) e = ma::launch_norm_quant<4, 32, false>(p, sms, st);

@@ -23,6 +23,7 @@ namespace ma {
 namespace {
 
 constexpr int kRaThreads = 128;
+constexpr int kRaGroups = 4;                      // groups of four heads of a warp
 
 __device__ __forceinline__ float ra_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float ra_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
@@ -30,6 +31,14 @@ __device__ __forceinline__ uint32_t ra_pack(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// read once; the asm keeps its place before the look-up
+__device__ __forceinline__ uint4 ra_load(const uint16_t* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
 }
 
 struct RopeAppend {
@@ -40,19 +49,40 @@ struct RopeAppend {
   int* dropped;                                   // (may be null)
   long long q_tok, q_head, k_tok, k_head, v_tok, v_head, out_tok, out_head, table_pitch;
   int num_batch, rows, H, Hkv, num_pages, width;
-  int parts, part_heads;                          // warps of a token, heads of each (a multiple of 4)
+  int parts;                                      // warps of a token
 };
 
-// The last sequence that starts at or before row t: 32 probes at a time.  (Sequences without new rows
-// start where their successor does, so the last one is the one that has the row.)
-__device__ __forceinline__ int sequence_of(const int* cu_q, int num_batch, int t, int lane) {
-  int lo = 0, n = num_batch;
-  while (n > 1) {
-    const int at = lane * search_step(n);
-    const unsigned before = __ballot_sync(0xffffffffu, at < n && cu_q[lo + (at < n ? at : 0)] <= t);
-    search_take(__popc(before), &lo, &n);
+struct Place {
+  int pos, page;                                  // -1: none
+};
+
+// Where row t goes.  The sequence is the last one that starts at or before the row, looked for with 32
+// probes at a time (sequences without new rows start where their successor does, so the last one is the one
+// that has the row).  A batch that fits a warp takes lengths along with the starts: one trip to memory less
+// before the page is known.
+__device__ __forceinline__ Place place_of(const RopeAppend& p, const int* cu_q, int t, int lane) {
+  Place at;
+  int b = 0, q0, q1, len;
+  if (p.num_batch < 32) {
+    const int start = cu_q[min(lane, p.num_batch)], n = p.lens[min(lane, p.num_batch - 1)];
+    b = max(__popc(__ballot_sync(0xffffffffu, lane < p.num_batch && start <= t)), 1) - 1;
+    q0 = __shfl_sync(0xffffffffu, start, b);
+    q1 = __shfl_sync(0xffffffffu, start, b + 1);
+    len = __shfl_sync(0xffffffffu, n, b);
+  } else {
+    int n = p.num_batch;
+    while (n > 1) {
+      const int i = lane * search_step(n);
+      const unsigned before = __ballot_sync(0xffffffffu, i < n && cu_q[b + (i < n ? i : 0)] <= t);
+      search_take(__popc(before), &b, &n);
+    }
+    q0 = cu_q[b];
+    q1 = cu_q[b + 1];
+    len = p.lens[b];
   }
-  return lo;
+  at.pos = position_of(t, q0, q1, len);
+  at.page = page_of(at.pos, p.table + b * p.table_pitch, p.width, p.num_pages);
+  return at;
 }
 
 __global__ void __launch_bounds__(kRaThreads) rope_append_kernel(const __grid_constant__ RopeAppend p) {
@@ -61,22 +91,35 @@ __global__ void __launch_bounds__(kRaThreads) rope_append_kernel(const __grid_co
   const int lane = threadIdx.x & 31;
   const long long unit = static_cast<long long>(blockIdx.x) * (kRaThreads / 32) + (threadIdx.x >> 5);
   const int t = static_cast<int>(unit / p.parts), part = static_cast<int>(unit % p.parts);
+  if (t >= p.rows) return;
   const int* cu_q = from_here(p.cu_q);
-  if (t >= p.rows || t >= cu_q[p.num_batch]) return;         // rows behind the last sequence: left alone
-  const int b = sequence_of(cu_q, p.num_batch, t, lane);
-  const int pos = position_of(t, cu_q[b], cu_q[b + 1], p.lens[b]);
-  const int page = page_of(pos, p.table + b * p.table_pitch, p.width, p.num_pages);
-  const bool stored = page >= 0;
-  if (part == 0 && lane == 0 && !stored && p.dropped) atomicAdd(p.dropped, 1);
-  if (pos < 0) return;
-
   const int sub = lane >> 3, dim = (lane & 7) * 8;
+  const int first = part * (4 * kRaGroups) + sub, all = p.H + 2 * p.Hkv;
+
+  // What this lane takes from its heads is on its way (rows behind the last sequence are the caller's too)
+  // while the row's place is looked up.
+  uint4 lo[kRaGroups], hi[kRaGroups];
+#pragma unroll
+  for (int g = 0; g < kRaGroups; ++g) {
+    const int h = first + 4 * g;
+    if (h >= all) break;
+    const int j = h < p.H ? h : h - p.H < p.Hkv ? h - p.H : h - p.H - p.Hkv;
+    const uint16_t* src = h < p.H ? p.q + t * p.q_tok + j * p.q_head
+                                  : h - p.H < p.Hkv ? p.k + t * p.k_tok + j * p.k_head : p.v + t * p.v_tok + j * p.v_head;
+    lo[g] = ra_load(src + dim);
+    hi[g] = ra_load(src + dim + 64);
+  }
+  if (t >= cu_q[p.num_batch]) return;              // rows behind the last sequence: left alone
+  const Place at = place_of(p, cu_q, t, lane);
+  if (part == 0 && lane == 0 && at.page < 0 && p.dropped) atomicAdd(p.dropped, 1);
+  if (at.pos < 0) return;
+
   float c[8], s[8];
   {
     float cs[2], sn[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const double turns = static_cast<double>(pos) *
+      const double turns = static_cast<double>(at.pos) *
                            (static_cast<double>(p.inv_freq[dim + 2 * sub + i]) * 0.15915494309189533577);
       sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn[i], &cs[i]);
     }
@@ -86,26 +129,19 @@ __global__ void __launch_bounds__(kRaThreads) rope_append_kernel(const __grid_co
       s[i] = __shfl_sync(0xffffffffu, sn[i & 1], (lane & 7) + 8 * (i >> 1));
     }
   }
-  const long long slot = static_cast<long long>(page) * 128 + (pos & 127);
-  const int all = p.H + 2 * p.Hkv, from = part * p.part_heads;
-  const int to = min(all, from + p.part_heads);
-  for (int h = from + sub; h < to; h += 4) {
-    const uint16_t* src;
-    uint16_t* dst;
-    bool turn = true;
-    if (h < p.H) {
-      src = p.q + t * p.q_tok + h * p.q_head;
-      dst = p.out + t * p.out_tok + h * p.out_head;
-    } else {
-      if (!stored) continue;
-      turn = h < p.H + p.Hkv;
-      const int j = turn ? h - p.H : h - p.H - p.Hkv;
-      src = turn ? p.k + t * p.k_tok + j * p.k_head : p.v + t * p.v_tok + j * p.v_head;
-      dst = (turn ? p.k_cache : p.v_cache) + (slot * p.Hkv + j) * 128;
+  const long long slot = static_cast<long long>(at.page) * 128 + (at.pos & 127);
+#pragma unroll
+  for (int g = 0; g < kRaGroups; ++g) {
+    const int h = first + 4 * g;
+    if (h >= all) break;
+    uint16_t* dst = p.out + t * p.out_tok + h * p.out_head;
+    const bool turn = h < p.H + p.Hkv;
+    if (h >= p.H) {
+      if (at.page < 0) break;
+      dst = (turn ? p.k_cache : p.v_cache) + (slot * p.Hkv + (turn ? h - p.H : h - p.H - p.Hkv)) * 128;
     }
-    uint4 lo = *reinterpret_cast<const uint4*>(src + dim), hi = *reinterpret_cast<const uint4*>(src + dim + 64);
     if (turn) {
-      const uint32_t lv[4] = {lo.x, lo.y, lo.z, lo.w}, hv[4] = {hi.x, hi.y, hi.z, hi.w};
+      const uint32_t lv[4] = {lo[g].x, lo[g].y, lo[g].z, lo[g].w}, hv[4] = {hi[g].x, hi[g].y, hi[g].z, hi[g].w};
       uint32_t ol[4], oh[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -113,11 +149,11 @@ __global__ void __launch_bounds__(kRaThreads) rope_append_kernel(const __grid_co
         ol[j] = ra_pack(a0 * c[2 * j] - b0 * s[2 * j], a1 * c[2 * j + 1] - b1 * s[2 * j + 1]);
         oh[j] = ra_pack(b0 * c[2 * j] + a0 * s[2 * j], b1 * c[2 * j + 1] + a1 * s[2 * j + 1]);
       }
-      lo = make_uint4(ol[0], ol[1], ol[2], ol[3]);
-      hi = make_uint4(oh[0], oh[1], oh[2], oh[3]);
+      lo[g] = make_uint4(ol[0], ol[1], ol[2], ol[3]);
+      hi[g] = make_uint4(oh[0], oh[1], oh[2], oh[3]);
     }
-    *reinterpret_cast<uint4*>(dst + dim) = lo;
-    *reinterpret_cast<uint4*>(dst + dim + 64) = hi;
+    *reinterpret_cast<uint4*>(dst + dim) = lo[g];
+    *reinterpret_cast<uint4*>(dst + dim + 64) = hi[g];
   }
 }
 
@@ -159,10 +195,7 @@ extern "C" int ma_rope_append(const ma_rope_append_args* a, void* stream) {
   p.table_pitch = a->table_pitch;
   p.num_batch = a->num_batch; p.rows = a->rows; p.H = a->H_local; p.Hkv = a->H_kv;
   p.num_pages = a->num_pages; p.width = a->table_width;
-  const int groups = (a->H_local + 2 * a->H_kv + 3) / 4;               // of four heads
-  const int each = 4;                                                  // groups of a warp
-  p.parts = (groups + each - 1) / each;
-  p.part_heads = each * 4;
+  p.parts = (a->H_local + 2 * a->H_kv + 4 * ma::kRaGroups - 1) / (4 * ma::kRaGroups);
   const long long ctas = (static_cast<long long>(p.rows) * p.parts + ma::kRaThreads / 32 - 1) / (ma::kRaThreads / 32);
   if (ctas > 0x7fffffffLL) return MA_ERR_CAPACITY;
   const cudaError_t e = ma::launch_behind(ma::rope_append_kernel, static_cast<int>(ctas), ma::kRaThreads, 0,
