@@ -67,9 +67,17 @@ dequant_kernel(const int8_t* q_, const float* scale_, T* out_, long long q_pitch
     for (int u = 0; u < kDqRows; ++u)
       if (row + u * step < rows) {
         s[u] = scale[row + u * step];
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w)
-                     : "l"(q + (row + u * step) * q_pitch + c * 16) : "memory");     // (rows are 16-byte multiples)
+        const int8_t* from = q + (row + u * step) * q_pitch + c * 16;
+        if (c * 16 + 16 <= cols) {
+          asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w) : "l"(from) : "memory");
+        } else {                             // (what is behind a row's last column may not be there)
+          uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c * 16 + i < cols) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(from[i])) << (8 * (i & 3));
+          v[u] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
 #pragma unroll
     for (int u = 0; u < kDqRows; ++u) {

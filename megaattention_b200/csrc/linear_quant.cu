@@ -696,8 +696,9 @@ int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms,
     const Form f = narrow_form(p, tn, sms);
     if (p.tokens <= 32 || f.time <= wide_form(p, sms).time) {
       if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
-      // an SM that has one CTA only gives it all of its shared memory (48 x 16384 x 2304: 12.5 us for 14.3)
-      const bool deep = f.tiles <= sms;
+      // an SM that has one CTA only gives it all of its shared memory (48 x 16384 x 2304: 12.4 us for 14.3);
+      // clusters of three and more find no room on some SMs
+      const bool deep = f.tiles <= (f.splits > 2 ? sms * 88 / 100 : sms);
       switch (tn) {
         case 16: return deep ? launch_narrow<16, 11>(a, p, f.splits, dev, stream) : launch_narrow<16, 6>(a, p, f.splits, dev, stream);
         case 32: return deep ? launch_narrow<32, 10>(a, p, f.splits, dev, stream) : launch_narrow<32, 5>(a, p, f.splits, dev, stream);

@@ -92,5 +92,7 @@ def residual_rmsnorm_int8(ws, residual, weight, eps: float = 1e-6, *, inplace: b
     assert meta is not None, "no layer has been set on this workspace"
     tokens = int(meta.cu_seqlens_q[-1])
     tiles = (ws.cu_q.data_ptr(), ws.fa_b.data_ptr(), ws.fa_mb.data_ptr())
-    return _queue(ws.csym.data_ptr(), ws.num_out * 128, tokens, int(meta.num_row_tiles), ws.hidden, weight, eps,
-                  residual, inplace, out, scale, ws.dev, tiles, ws._stream().cuda_stream)
+    assert residual is not None
+    with ws._on_stream():                  # (the results' memory is the workspace's stream's too)
+        return _queue(ws.csym.data_ptr(), ws.num_out * 128, tokens, int(meta.num_row_tiles), ws.hidden, weight, eps,
+                      residual, inplace, out, scale, ws.dev, tiles, ws._stream().cuda_stream)

@@ -81,6 +81,7 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens
         o_tok, o_head, o_one = out.stride()
         assert out.shape == shape and out.dtype is BF16 and out.get_device() == at and o_one == 1 and \
             not o_at & 15 and not (o_tok | o_head) & 7, "out: as q"
+        assert (o_tok >= 128 or tokens == 1) and (o_head >= 128 or H == 1), "heads of out overlap"
     d_at = 0
     if dropped is not None:
         assert dropped.shape == (1,) and dropped.dtype is I32 and dropped.get_device() == at, "dropped: [1] int32"
