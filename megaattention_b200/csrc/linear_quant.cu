@@ -360,6 +360,12 @@ __device__ __forceinline__ float4 ld_shared_f32x4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 struct WideTiles {
   int m, n, total, stored;                   // stored: the output takes TMA stores (16-byte rows)
 };
@@ -371,18 +377,21 @@ __device__ __forceinline__ void tile_at(const WideTiles& t, int i, int* m, int* 
   *m = g * kGroupM + r - *n * gm;
 }
 
-// 32 sums of a row to 32 outputs.
-__device__ __forceinline__ void scale_chunk(const uint32_t (&r)[32], float xs, uint32_t cols, uint32_t bias_at,
-                                            bool biased, float (&v)[32]) {
+// 32 sums of a row to 32 outputs, two at a time.
+template <bool BIASED>
+__device__ __forceinline__ void scale_columns(const uint32_t (&r)[32], uint64_t xs, uint32_t cols, uint32_t bias_at,
+                                              float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 s = ld_shared_f32x4(cols + j * 4);
     float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (biased) b = ld_shared_f32x4(cols + bias_at + j * 4);
-    v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])) * xs, s.x, b.x);
-    v[j + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + 1])) * xs, s.y, b.y);
-    v[j + 2] = fmaf(static_cast<float>(static_cast<int>(r[j + 2])) * xs, s.z, b.z);
-    v[j + 3] = fmaf(static_cast<float>(static_cast<int>(r[j + 3])) * xs, s.w, b.w);
+    if (BIASED) b = ld_shared_f32x4(cols + bias_at + j * 4);
+    const uint64_t lo = mul_f32x2(pack_f32x2(static_cast<float>(static_cast<int>(r[j])),
+                                             static_cast<float>(static_cast<int>(r[j + 1]))), xs);
+    const uint64_t hi = mul_f32x2(pack_f32x2(static_cast<float>(static_cast<int>(r[j + 2])),
+                                             static_cast<float>(static_cast<int>(r[j + 3]))), xs);
+    unpack_f32x2(fma_f32x2(lo, pack_f32x2(s.x, s.y), pack_f32x2(b.x, b.y)), v[j], v[j + 1]);
+    unpack_f32x2(fma_f32x2(hi, pack_f32x2(s.z, s.w), pack_f32x2(b.z, b.w)), v[j + 2], v[j + 3]);
   }
 }
 // 32 columns of this lane's row into the warp's staging: rows of ROW bytes, the columns from byte `at`, 16-byte
@@ -541,6 +550,7 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
       const int row0 = tm * 256 + static_cast<int>(rank) * 128 + (w & 3) * 32, n0 = tn * BN;
       const int rows = min(32, p.tokens - row0);             // (none or less: beyond the last token)
       const float xs = lane < rows ? p.x_scale[row0 + lane] : 0.f;
+      const uint64_t xs2 = pack_f32x2(xs, xs);
       const uint32_t cols = ring + S::kCols + acc * (2 * BN * 4);
       if (e < BN) {
         const int n = n0 + e;
@@ -569,7 +579,8 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         const int n = n0 + first + c * 32, chunk = n / kChunk * kChunk;
         if (rows <= 0 || n >= p.width) continue;                       // (the same for the warp)
         float v[32];
-        scale_chunk(r[c & 1], xs, cols + (first + c * 32) * 4, BN * 4, p.bias != nullptr, v);
+        if (p.bias) scale_columns<true>(r[c & 1], xs2, cols + (first + c * 32) * 4, BN * 4, v);
+        else scale_columns<false>(r[c & 1], xs2, cols + (first + c * 32) * 4, BN * 4, v);
         if (n == chunk) {                    // (the staging is free again once the store before has read it)
           if (lane == 0) tma_store_wait_read();
           __syncwarp();
