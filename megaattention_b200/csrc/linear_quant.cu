@@ -707,9 +707,10 @@ int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms,
     const Form f = narrow_form(p, tn, sms);
     if (p.tokens <= 32 || f.time <= wide_form(p, sms).time) {
       if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
-      // an SM that has one CTA only gives it all of its shared memory (48 x 16384 x 2304: 12.4 us for 14.3);
-      // clusters of three and more find no room on some SMs
-      const bool deep = f.tiles <= (f.splits > 2 ? sms * 88 / 100 : sms);
+      // an SM that has one CTA only gives it all of its shared memory, where its part is long enough to fill it
+      // (48 x 16384 x 2304: 12.4 us for 14.3; 16 x 4096 x 4096, 8 blocks a part: 7.7 for 7.2); clusters of three
+      // and more find no room on some SMs
+      const bool deep = f.tiles <= (f.splits > 2 ? sms * 88 / 100 : sms) && p.inner >= 16 * kSlab * f.splits;
       switch (tn) {
         case 16: return deep ? launch_narrow<16, 11>(a, p, f.splits, dev, stream) : launch_narrow<16, 6>(a, p, f.splits, dev, stream);
         case 32: return deep ? launch_narrow<32, 10>(a, p, f.splits, dev, stream) : launch_narrow<32, 5>(a, p, f.splits, dev, stream);
