@@ -348,8 +348,10 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
       ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
+// An arrival on a barrier of either CTA, for what tcgen05 fences order.  (With release semantics at cluster
+// scope it waited for the thread's stores, 1200 to 2700 cycles of a tile's epilogue.)
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
   asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
@@ -394,21 +396,13 @@ __device__ __forceinline__ void scale_columns(const uint32_t (&r)[32], uint64_t 
     unpack_f32x2(fma_f32x2(hi, pack_f32x2(s.z, s.w), pack_f32x2(b.z, b.w)), v[j + 2], v[j + 3]);
   }
 }
-// 32 columns of this lane's row into the warp's staging: rows of ROW bytes, the columns from byte `at`, 16-byte
-// pieces swizzled as the output's tensor map has it.
-template <bool F32, int ROW>
-__device__ __forceinline__ void put_columns(const float (&v)[32], uint32_t buffer, int at, int lane) {
+// This lane's row into the warp's staging: ROW bytes, 16-byte pieces swizzled as the output's tensor map has it.
+template <int ROW>
+__device__ __forceinline__ void put_row(const uint32_t* u, uint32_t staging, int lane) {
   const uint32_t flip = ROW == 128 ? lane & 7 : (lane >> 1) & 3;
 #pragma unroll
-  for (int j = 0; j < (F32 ? 8 : 4); ++j) {
-    const uint32_t to = buffer + lane * ROW + (((at >> 4) + j) ^ flip) * 16;
-    if (F32)
-      st_shared_v4(to, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
-                   __float_as_uint(v[4 * j + 3]));
-    else
-      st_shared_v4(to, pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                   pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-  }
+  for (int j = 0; j < ROW / 16; ++j)
+    st_shared_v4(staging + lane * ROW + ((j ^ flip) << 4), u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
 }
 // 32 columns of 32 rows by elements, two rows at a time: where rows do not start at 16 bytes, and a row's last
 // columns (TMA writes 16 bytes at a time, beyond the last column too).
@@ -564,7 +558,7 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
       if (!ok) continue;
       tc_fence_after();
       const uint32_t taddr = tmem + acc * BN + first + (static_cast<uint32_t>((w & 3) * 32) << 16);
-      uint32_t r[2][32];
+      uint32_t r[2][32], u[S::kRow / 4];       // (u: a staged row)
       tmem_ld32(taddr, r[0]);
 #pragma unroll
       for (int c = 0; c < BN / 64; ++c) {
@@ -581,13 +575,21 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         float v[32];
         if (p.bias) scale_columns<true>(r[c & 1], xs2, cols + (first + c * 32) * 4, BN * 4, v);
         else scale_columns<false>(r[c & 1], xs2, cols + (first + c * 32) * 4, BN * 4, v);
-        if (n == chunk) {                    // (the staging is free again once the store before has read it)
+        constexpr int kWords = F32 ? 32 : 16;          // of 32 columns
+        const bool whole = tiles.stored && chunk + kChunk <= p.width;
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < kWords; ++j)
+            u[c * kWords % (S::kRow / 4) + j] = F32 ? __float_as_uint(v[j]) : pack_bf16x2(v[2 * j % 32], v[(2 * j + 1) % 32]);
+        }
+        // (the staging is written as late as can be: the store before has to have read it)
+        if (!whole || n + 32 == chunk + kChunk) {
           if (lane == 0) tma_store_wait_read();
           __syncwarp();
         }
-        if (tiles.stored && chunk + kChunk <= p.width) {
-          put_columns<F32, S::kRow>(v, staging, (n - chunk) * kItem, lane);
+        if (whole) {
           if (n + 32 == chunk + kChunk) {    // TMA leaves out rows beyond the last
+            put_row<S::kRow>(u, staging, lane);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
