@@ -65,6 +65,11 @@ __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
+// The same for what needs no order of memory: that a CTA's shared memory lives on, or barriers that a fence of
+// their own has published.  (With release it waits for the thread's stores: 1500 to 2500 cycles at the end.)
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -78,9 +83,10 @@ __device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ int2 ld_peer(uint32_t addr) {
-  int2 v;
-  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+__device__ __forceinline__ int4 ld_peer(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
 
@@ -106,6 +112,10 @@ constexpr int kWBytes = 128 * kSlab;
 // tokens does not run a 128-row tile of them.  One tile of 128 channels x TN tokens per cluster; its CTAs
 // take a share of K each, and add their sums through each other's shared memory: integers, so the
 // order does not show.
+constexpr int kMaxSplits = 6;                // parts of K, the CTAs of a cluster
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+
 template <int TN, int STAGES>
 struct Narrow {
   static constexpr int kStage = kWBytes + TN * kSlab;
@@ -185,84 +195,89 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     }
     __syncwarp();
   }
-  // Two channels a thread in the end; their scales and the tokens' are fetched under the loads.
-  const int valid = min(TN, p.tokens - m0);
-  const int n = n0 + (tid & 63) * 2;
-  float ws[2] = {0.f, 0.f}, bias[2] = {0.f, 0.f};
+  // Four channels a lane in the end; their scales and the tokens' are fetched under the loads.
+  const int lane = tid & 31, valid = min(TN, p.tokens - m0), n = n0 + lane * 4;
+  float ws[4], bias[4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (n + j < p.width) {
-      ws[j] = p.w_scale[n + j];
-      if (p.bias) bias[j] = __uint_as_float(static_cast<uint32_t>(p.bias[n + j]) << 16);
-    }
+  for (int j = 0; j < 4; ++j) {
+    ws[j] = n + j < p.width ? p.w_scale[n + j] : 0.f;
+    bias[j] = p.bias && n + j < p.width ? __uint_as_float(static_cast<uint32_t>(p.bias[n + j]) << 16) : 0.f;
+  }
   for (int c = tid; c < valid; c += 128) s_xs[c] = p.x_scale[m0 + c];
   wait_bounded(done, 0, 0x13);
   tc_fence_after();
   __syncthreads();
 
   // Thread t holds channel t: its sums go to [token][channel] of this CTA's ring.
-  for (int c0 = 0; c0 < valid; c0 += 16) {
-    uint32_t r[16];
-    tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c0, r);
+  {
+    constexpr int kCol = TN < 32 ? 16 : 32;
+    uint32_t r[TN / kCol][kCol];
+#pragma unroll
+    for (int i = 0; i < TN / kCol; ++i) tmem_ld_columns(tmem + (static_cast<uint32_t>(warp * 32) << 16) + i * kCol, r[i]);
     tc_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring + ((c0 + i) * 128 + tid) * 4), "r"(r[i]) : "memory");
+    for (int i = 0; i < TN; ++i)
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring + (i * 128 + tid) * 4), "r"(r[i / kCol][i % kCol]) : "memory");
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 2) tmem_dealloc(tmem, kCols);
   if (splits > 1) { cluster_arrive(); cluster_wait(); }
 
-  // Every CTA adds up its share of the tokens: 64 threads a token, four tokens of each half in flight.
-  const int t1 = static_cast<int>(static_cast<long long>(valid) * (rank + 1) / splits);
+  // Every CTA adds up its share of the tokens, a warp two at a time, all parts of both in flight.
+  const int t1 = valid * (rank + 1) / splits;
   const int item = p.out_f32 ? 4 : 2;
-  const bool both = n + 1 < p.width && (p.out_pitch & 1) == 0 &&
-                    (reinterpret_cast<uint64_t>(p.out) & (2 * item - 1)) == 0;
+  const bool whole = n + 4 <= p.width && ((reinterpret_cast<uint64_t>(p.out) | static_cast<uint64_t>(p.out_pitch) * item) &
+                                          (4u * item - 1)) == 0;
   const uint32_t mine = splits > 1 ? 0 : cluster_rank();
-  for (int c = static_cast<int>(static_cast<long long>(valid) * rank / splits) + (tid >> 6); c < t1; c += 8) {
-    int2 sum[4];
+  for (int c = valid * rank / splits + warp; c < t1; c += 8) {
+    int4 part[2][kMaxSplits];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) sum[u] = make_int2(0, 0);
-#pragma unroll 2
-    for (int r = 0; r < splits; ++r) {
-      const uint32_t at = peer_smem(ring + (c * 128 + (tid & 63) * 2) * 4, mine + r);
+    for (int r = 0; r < kMaxSplits; ++r) {
+      const uint32_t at = peer_smem(ring + (c * 128 + lane * 4) * 4, mine + (r < splits ? r : 0));
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c + 2 * u < t1) {
-          const int2 v = ld_peer(at + u * 1024);
-          sum[u].x += v.x;
-          sum[u].y += v.y;
-        }
+      for (int u = 0; u < 2; ++u)
+        part[u][r] = r < splits && c + 4 * u < t1 ? ld_peer(at + u * 2048) : make_int4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (c + 2 * u >= t1) break;
-      const float xs = s_xs[c + 2 * u];
-      const float a = fmaf(static_cast<float>(sum[u].x) * xs, ws[0], bias[0]);
-      const float b = fmaf(static_cast<float>(sum[u].y) * xs, ws[1], bias[1]);
-      const long long o = static_cast<long long>(m0 + c + 2 * u) * p.out_pitch + n;
+    for (int u = 0; u < 2; ++u) {
+      if (c + 4 * u >= t1) break;
+      int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < kMaxSplits; ++r) {
+        sum[0] += part[u][r].x;
+        sum[1] += part[u][r].y;
+        sum[2] += part[u][r].z;
+        sum[3] += part[u][r].w;
+      }
+      const float xs = s_xs[c + 4 * u];
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = fmaf(static_cast<float>(sum[j]) * xs, ws[j], bias[j]);
+      const long long o = static_cast<long long>(m0 + c + 4 * u) * p.out_pitch + n;
       if (p.out_f32) {
         float* out = static_cast<float*>(p.out) + o;
-        if (both) {
-          *reinterpret_cast<float2*>(out) = make_float2(a, b);
+        if (whole) {
+          *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-          if (n < p.width) out[0] = a;
-          if (n + 1 < p.width) out[1] = b;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.width) out[j] = v[j];
         }
       } else {
         uint16_t* out = static_cast<uint16_t*>(p.out) + o;
-        const uint32_t v = pack_bf16x2(a, b);
-        if (both) {
-          *reinterpret_cast<uint32_t*>(out) = v;
+        const uint2 w = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        if (whole) {
+          *reinterpret_cast<uint2*>(out) = w;
         } else {
-          if (n < p.width) out[0] = static_cast<uint16_t>(v);
-          if (n + 1 < p.width) out[1] = static_cast<uint16_t>(v >> 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.width) out[j] = static_cast<uint16_t>((j < 2 ? w.x : w.y) >> (16 * (j & 1)));
         }
       }
     }
   }
-  if (splits > 1) { cluster_arrive(); cluster_wait(); }     // (peers read this CTA's sums until here)
+  if (splits > 1) { cluster_arrive_relaxed(); cluster_wait(); }     // (peers read this CTA's sums until here)
 }
 
 // A kernel's shared memory beyond 48 KB, allowed once per device (an attribute that outlasts the call; to
@@ -459,7 +474,7 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
   }
   tc_fence_before();
   __syncthreads();
-  cluster_arrive();                          // (the other CTA's barriers are set up)
+  cluster_arrive_relaxed();                  // (the other CTA's barriers are set up)
   cluster_wait();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
@@ -602,12 +617,12 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
       }
     }
-    if (lane == 0) tma_store_wait_all();
+    if (lane == 0) tma_store_wait_read();    // (the staging lives until its last store has read it)
     __syncwarp();
   }
   __syncthreads();
   tc_fence_before();
-  cluster_arrive();                          // (barriers and sums of a CTA are used by the other)
+  cluster_arrive_relaxed();                  // (barriers and sums of a CTA are used by the other)
   cluster_wait();
   tc_fence_after();
   if (warp == 2)
@@ -684,10 +699,10 @@ Form narrow_form(const LinearArgs& p, int tn, int sms) {
   const long long tiles = (p.width + 127LL) / 128 * ((p.tokens + tn - 1LL) / tn);
   const long long room = 2LL * sms * 92 / 100;
   Form best{0, 0, 0, 0};
-  for (int n : {1, 2, 3, 4, 6}) {
+  for (int n : {1, 2, 3, 4, kMaxSplits}) {
     if (n > blocks) break;
     const long long load = blocks * 340 / n;
-    const long long time = (tiles * n + room - 1) / room * ((load > 2040 ? load : 2040) + (n > 1 ? 1020 + 340 * n : 0));
+    const long long time = (tiles * n + room - 1) / room * ((load > 2040 ? load : 2040) + (n > 1 ? 600 + 200 * n : 0));
     if (n == 1 || time < best.time) best = {tiles * n, time, 0, n};
   }
   return best;
