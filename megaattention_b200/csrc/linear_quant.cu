@@ -736,7 +736,7 @@ int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms,
     }
   }
   const Form f = wide_form(p, sms);
-  if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
+  if (f.tiles > 0x7fff0000LL) return MA_ERR_CAPACITY;      // (tiles are counted in 32 bits, a round beyond the last)
   switch (f.width) {
     case 64: return launch_wide<64, 9>(a, p, sms, dev, stream);
     case 128: return launch_wide<128, 7>(a, p, sms, dev, stream);

@@ -97,6 +97,18 @@ def test_pitches_and_a_given_output(m):
             assert bool((rest == -7.0).all())
 
 
+@pytest.mark.parametrize("m,n", [(70000, 32768), (3, 500000)])
+def test_outputs_beyond_32_bits_of_elements_and_wide_ones(m, n):
+    from megaattention_b200.runtime import check_linear_status, linear_int8
+    g = torch.Generator().manual_seed(m)
+    x, w = _rows(m, 48, g), _rows(n, 48, g)
+    xs, ws = torch.rand(m, generator=g).cuda(), torch.rand(n, generator=g).cuda() / 1000
+    out = linear_int8(x, xs, w, ws)
+    at = torch.tensor(sorted({0, 1, m // 2, m - 2, m - 1}), device="cuda")
+    _check(out[at], x[at], xs[at], w, ws, None)
+    check_linear_status()
+
+
 def test_nothing_to_do_and_scales_that_are_not_finite():
     from megaattention_b200.runtime import linear_int8
     x, xs, w, ws, b = _case(20, 64, 48, True)

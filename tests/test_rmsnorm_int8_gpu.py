@@ -50,6 +50,21 @@ def test_packed_rows(tokens, hidden):
     assert same is r and torch.equal(q, q2) and torch.equal(scale, scale2) and torch.equal(new, r)
 
 
+def test_rows_beyond_32_bits_of_elements():
+    from megaattention_b200.runtime import dequantize_int8, rmsnorm_int8
+    tokens, hidden = 135000, 16384
+    x = torch.empty(tokens, hidden, dtype=torch.bfloat16, device="cuda")
+    rows, r, w = _inputs(7, hidden)
+    at = torch.tensor([0, 1, 65535, 131071, 131072, tokens - 2, tokens - 1], device="cuda")
+    x[at] = rows
+    q, scale = rmsnorm_int8(x, w)
+    _check(q[at], scale[at], rows, w, 1e-6)
+    for a in at.tolist():
+        x[a] = float("nan")
+    out = dequantize_int8(q, scale, out=x)
+    assert torch.equal(out[at], (q[at].float() * scale[at, None]).bfloat16())
+
+
 def test_no_rows():
     from megaattention_b200.runtime import rmsnorm_int8
     x, r, w = _inputs(0, 64)

@@ -168,6 +168,36 @@ def test_table_and_lengths_as_views():
     assert _check(c, got, kc, vc) == 0
 
 
+def test_a_place_beyond_32_bits_of_elements():
+    """Caches of 16500 pages of 8 heads: the last pages start beyond 2^31 elements."""
+    from megaattention_b200.runtime import rope_append
+    pages = 16500
+    kc, vc = (torch.empty(pages, 128, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    kc[-3:], vc[-3:] = 1, 1
+    c = _case([5, 140], [300, 140], 16, 8, seed=3)
+    c["table"] = [[0, 0, pages - 1], [pages - 2, pages - 3, 0]]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q, k, v = _split(c["qkv"].cuda(), 16, 8)
+    got = rope_append(q, k, v, kc, vc, torch.tensor(c["table"], **i32), torch.tensor(c["lens"], **i32),
+                      torch.tensor(c["cu"], **i32))
+    c["table"] = [[0, 0, 2], [1, 0, 0]]
+    c["k_cache"] = c["v_cache"] = torch.ones(3, 128, 8, 128, dtype=torch.bfloat16)
+    assert _check(c, got, kc[-3:], vc[-3:]) == 0
+
+
+def test_two_rows_with_the_same_place():
+    """Either row's key is there in the end, whole, and nothing else changed."""
+    c = _case([1, 1], [5, 5], 4, 1)
+    c["table"] = [[1, 0], [1, 0]]
+    got, kc, vc = _run(c)
+    outs = []
+    for rows in (0, 1):
+        d = dict(c, cu=[0, 1, 1] if rows == 0 else [0, 0, 1], qkv=c["qkv"][rows:rows + 1])
+        outs.append(_run(d))
+    assert any(torch.equal(kc, o[1]) for o in outs) and any(torch.equal(vc, o[2]) for o in outs)
+    assert torch.equal(got, torch.cat([o[0] for o in outs]))
+
+
 def test_refusals():
     from megaattention_b200.runtime import rope_append
     c = _case([3], [5], 4, 2)
