@@ -1,6 +1,17 @@
 // Matrix product of 8-bit integers with a scale for each token and each output channel, on the integer
 // tensor path (tcgen05.mma kind::i8, exact 32-bit sums in TMEM):
 //   out[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] + bias[n].
+// The sum is converted to fp32, scaled and biased there, and rounded once to the output's type.
+//
+// With few tokens the weights' way from memory bounds it (one byte per weight), with many the tensor cores
+// (8192 products per cycle and SM) and, in a long run, the power limit.  Two kernels, each in a few widths;
+// linear_dispatch at the end says which and why.  Device time in a chain of calls, inputs from memory:
+//   tokens x inner x width       time      of the measured copy rate / of twice the measured bf16 rate
+//       1 x  4096 x 10240      8.9 us      0.73 of the copy rate
+//      48 x 16384 x  2304     10.8 us      0.56
+//    1384 x  4096 x  1280     10.1 us      0.43 of the burst rate (3365 TOP/s)
+//   13400 x  4096 x 10240      351 us      0.95; back to back for a second 412 us, 0.98 of the sustained (2781)
+//   22600 x  4096 x 16384      937 us      0.96; 1102 us, 0.99
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -111,7 +122,8 @@ constexpr int kWBytes = 128 * kSlab;
 // The weights are the matrix instruction's 128 rows and TN tokens its columns, so that a handful of
 // tokens does not run a 128-row tile of them.  One tile of 128 channels x TN tokens per cluster; its CTAs
 // take a share of K each, and add their sums through each other's shared memory: integers, so the
-// order does not show.
+// order does not show.  Every CTA has 64 to 180 KB on their way; what is left beside the loads is the start
+// of a kernel and of its first load, the exchange, and the end (1 x 512 x 512 takes 2.7 us).
 constexpr int kMaxSplits = 6;                // parts of K, the CTAs of a cluster
 __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
@@ -330,6 +342,9 @@ int launch_narrow(const ma_linear_quant_args* a, const LinearArgs& p, int splits
 // the weight rows, and one issuer runs both tensor cores, so a byte of either operand is loaded once per
 // pair.  Persistent pairs walk the tiles, 8 tiles of tokens at a time so that what runs at once shares its
 // operands in L2; the sums are double-buffered in TMEM, so the epilogue of a tile runs under the next.
+// An SM takes in 64 bytes a cycle at most, which is what a tile of 256 channels asks for (32 KB per 512 cycles
+// of products); tiles of 512, single-buffered in two halves, ask for 48 and were slower (4096 x 4096 x 4096
+// 51 us for 48) until K is 16384 long (205 for 211).  4096 x 4096 x 4096: tensor cores 81 % busy, 48 us.
 template <int BN, int STAGES, bool F32>
 struct Wide {
   static constexpr int kA = 128 * kSlab, kB = BN / 2 * kSlab, kStage = kA + kB;
@@ -386,7 +401,7 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
 struct WideTiles {
   int m, n, total, stored;                   // stored: the output takes TMA stores (16-byte rows)
 };
-constexpr int kGroupM = 8;
+constexpr int kGroupM = 8;                   // tiles of tokens that are walked together
 __device__ __forceinline__ void tile_at(const WideTiles& t, int i, int* m, int* n) {
   const int per = kGroupM * t.n, g = i / per, r = i - g * per;
   const int gm = min(kGroupM, t.m - g * kGroupM);
@@ -684,12 +699,12 @@ int launch_wide(const ma_linear_quant_args* a, const LinearArgs& p, int sms, int
 // Which kernel, and in which form, by estimates of its time in nanoseconds (device time of a call in a chain
 // of calls, beside a start and an end that all of them have):
 //   few tokens: rounds of two CTAs per SM (92 % of them: clusters leave some over) times a part's loads; what
-//   the ring holds comes at once, and parts have to be exchanged.  1 x 4096 x 10240: 3 parts 9.8 us, 2 11.8,
-//   4 15.0; 1 x 1024 x 8192: 1 part 4.2, 2 4.7; 1 x 16384 x 2304: 6 parts 10.9, 4 11.5, 1 27;
-//   many tokens: rounds of a tile per pair of SMs; 4096 x 4096 x 4096: 256 channels 48 us, 128 53, 64 89;
-//   1384 x 4096 x 1280: 15.2, 11.5, 15.9; 777 x 1000 x 1001: 12.6, 8.7, 7.2.
-// Up to 32 tokens the first always, above 512 the second; in between 64 x 4096 x 4096 takes 9.9 by the first
-// and 10.4 by the second, 256 x 4096 x 4096 12.6 and 10.8, 192 x 16384 x 2304 17.7 and 25.7.
+//   the ring holds comes at once, and parts have to be exchanged.  1 x 4096 x 10240: 3 parts 9.0 us, 2 11.0,
+//   4 13.4; 4 x 300 x 20000: 1 part 4.6, 2 7.7; 10 x 16384 x 2304: 6 parts 9.7, 4 10.7, 3 11.4;
+//   many tokens: rounds of a tile per pair of SMs; 4096 x 4096 x 4096: 256 channels 48 us, 128 54, 64 87;
+//   1384 x 4096 x 1280: 14.4, 10.5, 14.9; 777 x 1000 x 1001: 11.7, 7.9, 6.2.
+// Up to 32 tokens the first always, above 512 the second; in between 64 x 4096 x 4096 takes 8.4 by the first
+// and 9.3 by the second, 64 x 512 x 512 4.1 and 3.3, 300 x 16384 x 2304 19.1 and 25.4.
 struct Form {
   long long tiles, time;
   int width, splits;                         // channels of a tile, or parts of K
@@ -725,7 +740,7 @@ int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms,
     if (p.tokens <= 32 || f.time <= wide_form(p, sms).time) {
       if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
       // an SM that has one CTA only gives it all of its shared memory, where its part is long enough to fill it
-      // (48 x 16384 x 2304: 12.4 us for 14.3; 16 x 4096 x 4096, 8 blocks a part: 7.7 for 7.2); clusters of three
+      // (48 x 16384 x 2304: 10.9 us for 12.9; 16 x 4096 x 4096, 8 blocks a part: 6.7 for 6.1); clusters of three
       // and more find no room on some SMs
       const bool deep = f.tiles <= (f.splits > 2 ? sms * 88 / 100 : sms) && p.inner >= 16 * kSlab * f.splits;
       switch (tn) {

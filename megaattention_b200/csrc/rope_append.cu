@@ -8,10 +8,12 @@
 // The angle reaches 1e5 radians and more, where 32 bits resolve 0.004: it is reduced in 64 bits, as turns
 // p (w_d / 2 pi) less their nearest integer, and sine and cosine are taken of the remainder.
 //
-// HBM bound: q is read and written, k and v read and written once.  A warp takes a group of a token's
-// heads.  Lane l has dimensions 8 (l % 8) + 0..7 and their partners 64 further on, of head l / 8 of four
-// at a time, so that the eight sines and cosines that it needs are the same for every head: it computes
-// two of each, and the other lanes of its dimensions the rest.  No shared memory and no barrier.
+// HBM bound: q is read and written, k and v read and written once.  22600 tokens of 64 + 8 heads: 143 us, 6.46
+// TB/s, the measured copy rate; 1384 tokens of 16 + 2 heads 4.8 us (7.4 with the place looked up before the
+// first load), 64 tokens of 8 + 1 heads 3.0.  A warp takes sixteen of a token's heads.  Lane l has
+// dimensions 8 (l % 8) + 0..7 and their partners 64 further on, of head l / 8 of four at a time, so that the
+// eight sines and cosines that it needs are the same for every head: it computes two of each, and the other
+// lanes of its dimensions the rest.  No shared memory and no barrier.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
