@@ -57,7 +57,7 @@ def test_large_sizes(m, k, n, bias):
     check_linear_status()
 
 
-@pytest.mark.parametrize("m,k,n", [(3, 131071, 40), (300, 131071, 200)])
+@pytest.mark.parametrize("m,k,n", [(3, 131071, 40), (300, 131071, 200), (600, 131071, 200)])
 def test_the_longest_sums_are_exact(m, k, n):
     """-128 throughout: 131071 * 2^14 is the largest sum that can come up, just below 2^31."""
     from megaattention_b200.runtime import linear_int8
@@ -158,6 +158,26 @@ def test_eight_bits_as_the_values_they_stand_for(rows, cols):
     assert dequantize_int8(q[:0], s[:0]).shape == (0, cols)
     with pytest.raises(AssertionError):
         dequantize_int8(q.float(), s)
+
+
+@pytest.mark.parametrize("tokens", [8, 700])
+def test_weights_written_by_the_kernel_before(tokens):
+    """The projection starts while the kernel before it ends, and sends for its first weights then: a weight
+    that this very kernel writes is the new one all the same, every time."""
+    from megaattention_b200.runtime import linear_int8, rmsnorm_int8
+    g = torch.Generator().manual_seed(tokens)
+    x, xs = _rows(tokens, 2048, g), torch.rand(tokens, generator=g).cuda()
+    ones = torch.ones(2048, dtype=torch.bfloat16, device="cuda")
+    keys = [torch.randn(3000, 2048, generator=g).bfloat16().cuda() for _ in range(4)]
+    want = [linear_int8(x, xs, *rmsnorm_int8(k, ones)) for k in keys]
+    torch.cuda.synchronize()
+    w, ws = torch.empty(3000, 2048, dtype=torch.int8, device="cuda"), torch.empty(3000, device="cuda")
+    outs = []
+    for i in range(40):
+        rmsnorm_int8(keys[i % 4], ones, out=w, scale=ws)
+        outs.append(linear_int8(x, xs, w, ws))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 4]) for i, o in enumerate(outs))
 
 
 def test_captured_calls_two_streams_and_equal_bits():

@@ -143,6 +143,29 @@ def test_tiles_of_the_fused_output_in_place():
         assert q2 is q
 
 
+def test_the_fused_output_from_another_stream():
+    """Runs on the workspace's stream, results allocated there, whatever stream is current."""
+    from megaattention_b200.metadata import build_row_desc
+    from megaattention_b200.runtime import FusedFaOprojArWorkspace, residual_rmsnorm_int8
+    meta = build_row_desc([128])
+    ws = FusedFaOprojArWorkspace.create(None, 1, 512, 2, 128, q_per_kv=2, max_tot_k=128, device="cuda:0")
+    ws.compile()
+    ws.set_meta(meta)
+    y, r, w = _inputs(128, 512)
+    ws.csym.copy_(y.view(ws.csym.shape))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        q, scale, new = residual_rmsnorm_int8(ws, r, w, 1e-5)
+        assert torch.cuda.current_stream() == side
+    ws._stream().synchronize()
+    _check(q, scale, y, w, 1e-5, r, new)
+    with pytest.raises(AssertionError):
+        residual_rmsnorm_int8(ws, r[:100], w)
+    with pytest.raises(AssertionError):
+        residual_rmsnorm_int8(ws, None, w)
+
+
 def test_refusals():
     from megaattention_b200.runtime import rmsnorm_int8
     x, r, w = _inputs(4, 64)
