@@ -344,7 +344,7 @@ int launch_narrow(const ma_linear_quant_args* a, const LinearArgs& p, int splits
 // operands in L2; the sums are double-buffered in TMEM, so the epilogue of a tile runs under the next.
 // An SM takes in 64 bytes a cycle at most, which is what a tile of 256 channels asks for (32 KB per 512 cycles
 // of products); tiles of 512, single-buffered in two halves, ask for 48 and were slower (4096 x 4096 x 4096
-// 51 us for 48) until K is 16384 long (205 for 211).  4096 x 4096 x 4096: tensor cores 81 % busy, 48 us.
+// 50 us for 48) until K is 16384 long (208 for 218).  4096 x 4096 x 4096: tensor cores 81 % busy, 48 us.
 template <int BN, int STAGES, bool F32>
 struct Wide {
   static constexpr int kA = 128 * kSlab, kB = BN / 2 * kSlab, kStage = kA + kB;
