@@ -434,29 +434,79 @@ __device__ __forceinline__ void put_row(const uint32_t* u, uint32_t staging, int
   for (int j = 0; j < ROW / 16; ++j)
     st_shared_v4(staging + lane * ROW + ((j ^ flip) << 4), u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
 }
-// 32 columns of 32 rows by elements, two rows at a time: where rows do not start at 16 bytes, and a row's last
-// columns (TMA writes 16 bytes at a time, beyond the last column too).
-template <bool F32>
-__device__ __forceinline__ void store_elements(const LinearArgs& p, const float (&v)[32], uint32_t buffer, int n,
-                                               int row0, int rows, int lane) {
+// Staged rows to rows that do not start at 16 bytes, and a row's last columns (TMA writes 16 bytes at a time,
+// beyond the last column too): 16 bytes at a time where the output has them, ROW / 16 lanes a row, and what is
+// left on either side by elements.  `bytes` of each of `rows` rows.  A batch is read before any of it is
+// written: one at a time, every row waited for its words.
+template <int ITEM, int ROW>
+__device__ __forceinline__ void copy_rows(uint32_t staging, char* out, long long pitch, int rows, int bytes, int lane) {
+  constexpr int kPieces = ROW / 16, kRows = 32 / kPieces, kBatch = 4;
+  auto piece = [&](int row, int j) {         // where a staged row's j-th 16 bytes are
+    return staging + row * ROW + (((j & (kPieces - 1)) ^ (ROW == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+  };
+  {
+    const int j = lane % kPieces;
+    const long long step = pitch * kRows;
+    char* to = out + lane / kPieces * pitch;
+#pragma unroll 1
+    for (int r0 = lane / kPieces; r0 < rows; r0 += kBatch * kRows, to += kBatch * step) {
+      uint32_t w[kBatch][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    __syncwarp();
+      for (int i = 0; i < kBatch; ++i) {     // (row 31 and below, whatever `rows` is)
+        const int r = (r0 + i * kRows) & 31;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) st_shared_f32(buffer + (lane * 16 + (j ^ (lane & 15))) * 4, v[16 * h + j]);
-    __syncwarp();
-    const int col = n + 16 * h + (lane & 15);
-    if (col >= p.width) continue;
-#pragma unroll 8
-    for (int r = lane >> 4; r < rows; r += 2) {
-      float x;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buffer + (r * 16 + ((lane & 15) ^ (r & 15))) * 4) : "memory");
-      const long long o = static_cast<long long>(row0 + r) * p.out_pitch + col;
-      if (F32) static_cast<float*>(p.out)[o] = x;
-      else static_cast<uint16_t*>(p.out)[o] = static_cast<uint16_t>(pack_bf16x2(x, 0.f));
+        for (int h = 0; h < 2; ++h)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[i][4 * h]), "=r"(w[i][4 * h + 1]), "=r"(w[i][4 * h + 2]), "=r"(w[i][4 * h + 3])
+                       : "r"(piece(r, j + h)));
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        char* row = to + i * step;
+        const int head = -static_cast<int>(reinterpret_cast<uint64_t>(row)) & 15;
+        uint32_t* x = w[i];
+        if (head & 8) {
+#pragma unroll
+          for (int k = 0; k < 6; ++k) x[k] = x[k + 2];
+        }
+        if (head & 4) {
+#pragma unroll
+          for (int k = 0; k < 5; ++k) x[k] = x[k + 1];
+        }
+        if (ITEM == 2 && (head & 2)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = __funnelshift_r(x[k], x[k + 1], 16);
+        }
+        if (r0 + i * kRows < rows && head + j * 16 + 16 <= bytes)
+          *reinterpret_cast<uint4*>(row + head + j * 16) = make_uint4(x[0], x[1], x[2], x[3]);
+      }
     }
   }
-  __syncwarp();
+  constexpr int kSide = 16 / ITEM, kSideRows = 32 / (2 * kSide), kSides = 8;
+  const int e = lane % kSide * ITEM;
+  const bool left = lane % (2 * kSide) < kSide;
+  const long long step = pitch * kSideRows;
+  char* to = out + lane / (2 * kSide) * pitch;
+#pragma unroll 1
+  for (int r0 = lane / (2 * kSide); r0 < rows; r0 += kSides * kSideRows, to += kSides * step) {
+    uint32_t w[kSides];
+    int at[kSides];
+#pragma unroll
+    for (int i = 0; i < kSides; ++i) {
+      const int head = min(-static_cast<int>(reinterpret_cast<uint64_t>(to + i * step)) & 15, bytes);
+      at[i] = left ? e : head + ((bytes - head) & ~15) + e;
+      const uint32_t from = piece((r0 + i * kSideRows) & 31, at[i] >> 4) + (at[i] & 15);
+      if (ITEM == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(from));
+      else asm volatile("{\n\t.reg .u16 t;\n\tld.shared.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(w[i]) : "r"(from));
+      if (r0 + i * kSideRows >= rows || at[i] >= (left ? head : bytes)) at[i] = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kSides; ++i) {
+      if (at[i] < 0) continue;
+      if (ITEM == 4) *reinterpret_cast<uint32_t*>(to + i * step + at[i]) = w[i];
+      else *reinterpret_cast<uint16_t*>(to + i * step + at[i]) = static_cast<uint16_t>(w[i]);
+    }
+  }
 }
 
 template <int BN, int STAGES, bool F32>
@@ -601,34 +651,32 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
           if (lane == 0) mbar_arrive_peer(peer_smem(acc_empty + 8 * acc, 0));
         }
         const int n = n0 + first + c * 32, chunk = n / kChunk * kChunk;
-        if (rows <= 0 || n >= p.width) continue;                       // (the same for the warp)
+        if (rows <= 0 || chunk >= p.width) continue;                   // (the same for the warp)
         float v[32];
         if (p.bias) scale_columns<true>(r[c & 1], xs2, cols + (first + c * 32) * 4, BN * 4, v);
         else scale_columns<false>(r[c & 1], xs2, cols + (first + c * 32) * 4, BN * 4, v);
         constexpr int kWords = F32 ? 32 : 16;          // of 32 columns
-        const bool whole = tiles.stored && chunk + kChunk <= p.width;
-        if (whole) {
 #pragma unroll
-          for (int j = 0; j < kWords; ++j)
-            u[c * kWords % (S::kRow / 4) + j] = F32 ? __float_as_uint(v[j]) : pack_bf16x2(v[2 * j % 32], v[(2 * j + 1) % 32]);
-        }
+        for (int j = 0; j < kWords; ++j)
+          u[c * kWords % (S::kRow / 4) + j] = F32 ? __float_as_uint(v[j]) : pack_bf16x2(v[2 * j % 32], v[(2 * j + 1) % 32]);
+        if (n + 32 < chunk + kChunk) continue;
         // (the staging is written as late as can be: the store before has to have read it)
-        if (!whole || n + 32 == chunk + kChunk) {
-          if (lane == 0) tma_store_wait_read();
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+        put_row<S::kRow>(u, staging, lane);
+        if (tiles.stored && chunk + kChunk <= p.width) {     // TMA leaves out rows beyond the last
+          fence_proxy_async_smem();
           __syncwarp();
-        }
-        if (whole) {
-          if (n + 32 == chunk + kChunk) {    // TMA leaves out rows beyond the last
-            put_row<S::kRow>(u, staging, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&out_map, staging, chunk, row0);
-              tma_store_commit();
-            }
+          if (lane == 0) {
+            tma_store_2d(&out_map, staging, chunk, row0);
+            tma_store_commit();
           }
         } else {
-          store_elements<F32>(p, v, staging, n, row0, rows, lane);
+          __syncwarp();
+          copy_rows<kItem, S::kRow>(staging,
+                                    static_cast<char*>(p.out) + (static_cast<long long>(row0) * p.out_pitch + chunk) * kItem,
+                                    p.out_pitch * kItem, rows, min(kChunk, p.width - chunk) * kItem, lane);
+          __syncwarp();
         }
       }
     }
