@@ -1,0 +1,30 @@
+"""The operators' native calls (``csrc/calls.cpp``), built for the torch that is installed and bound to the
+library's entry points.  There is no fallback: without the module importing this raises.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import os
+
+import torch
+
+from . import _cabi, build as _build
+
+
+def _load():
+    if _build._stale(_build.LIB_CALLS):
+        try:
+            _build.build_calls()
+        except Exception as exc:  # no compiler on this machine: use what is there, if anything
+            if not os.path.exists(_build.LIB_CALLS):
+                raise ImportError(f"{os.path.basename(_build.LIB_CALLS)} is missing and cannot be built: {exc}")
+    from . import _calls
+    if _calls.torch_version != torch.__version__:
+        raise ImportError(f"{os.path.basename(_build.LIB_CALLS)} was built for torch {_calls.torch_version}, this is "
+                          f"{torch.__version__}: build it again")
+    _calls.bind(*(C.cast(getattr(_cabi.lib, name), C.c_void_p).value for name in (
+        "ma_rmsnorm_quant", "ma_linear_quant", "ma_dequant", "ma_rope_append", "ma_strerror")))
+    return _calls
+
+
+calls = _load()

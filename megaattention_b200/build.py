@@ -4,6 +4,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -19,18 +20,49 @@ SOURCES = ["fused_prefill.cu", "cabi.cu", "noalloc.cu", "residual_rmsnorm.cu", "
 HEADERS = ["ptx.cuh", "kparams.h", "launch.cuh", "paged.cuh", "append_place.h", os.path.join("..", "..", "include", "megaattn_b200.h")]
 
 
+# The operators' calls natively (csrc/calls.cpp): a Python module over torch's tensors, which hands the C ABI's
+# entry points plain pointers.  Host code only.
+LIB_CALLS = os.path.join(HERE, "_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+CALLS = ["calls.cpp", os.path.join("..", "..", "include", "megaattn_b200.h")]
+
+
 def _stale(lib: str = None) -> bool:
     lib = lib or LIB
     if not os.path.exists(lib):
         return True
     t = os.path.getmtime(lib)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
+    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in (CALLS if lib == LIB_CALLS else SOURCES + HEADERS))
 
 
 def build(force: bool = False, verbose: bool = False, audit: bool = False) -> str:
     """Compile ``csrc/*.cu`` into ``libmegaattn_b200.so`` (or, with ``audit``, into
     ``libmegaattn_b200_audit.so``) next to this file."""
     LIB = LIB_AUDIT if audit else globals()["LIB"]
+    nvcc = os.environ.get("NVCC", "nvcc")
+    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3",
+           "-std=c++17", "-Xcompiler", "-fPIC", "-shared"]
+    if verbose:
+        cmd += ["-Xptxas", "-v"]
+    if audit:
+        cmd += ["-DMA_AUDIT"]
+    return _compile(LIB, cmd + [os.path.join(CSRC, f) for f in SOURCES], force, verbose)
+
+
+def build_calls(force: bool = False) -> str:
+    """Compile ``csrc/calls.cpp`` against the torch that is installed."""
+    import torch
+    at = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f'-DMA_TORCH_VERSION="{torch.__version__}"', "-I" + sysconfig.get_paths()["include"],
+           "-I" + os.path.join(cuda, "include"), "-I" + os.path.join(at, "include"),
+           "-I" + os.path.join(at, "include", "torch", "csrc", "api", "include"), os.path.join(CSRC, "calls.cpp"),
+           "-L" + os.path.join(at, "lib"), "-Wl,-rpath," + os.path.join(at, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python"]
+    return _compile(LIB_CALLS, cmd, force)
+
+
+def _compile(LIB: str, cmd: list, force: bool, verbose: bool = False) -> str:
     if not force and not _stale(LIB):
         return LIB
     # Several processes (one per GPU under torchrun) may get here at once: one builds, into a
@@ -41,20 +73,12 @@ def build(force: bool = False, verbose: bool = False, audit: bool = False) -> st
         fcntl.flock(lock, fcntl.LOCK_EX)
         if not force and not _stale(LIB):
             return LIB
-        nvcc = os.environ.get("NVCC", "nvcc")
         tmp = f"{LIB}.{os.getpid()}.tmp"
-        cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3",
-               "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-o", tmp]
-        if verbose:
-            cmd += ["-Xptxas", "-v"]
-        if audit:
-            cmd += ["-DMA_AUDIT"]
-        cmd += [os.path.join(CSRC, f) for f in SOURCES]
-        res = subprocess.run(cmd, capture_output=True, text=True)
+        res = subprocess.run(cmd + ["-o", tmp], capture_output=True, text=True)
         if res.returncode != 0:
             if os.path.exists(tmp):
                 os.remove(tmp)
-            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n" + res.stdout + res.stderr)
         os.replace(tmp, LIB)
         if verbose:
             sys.stderr.write(res.stderr)
@@ -64,3 +88,4 @@ def build(force: bool = False, verbose: bool = False, audit: bool = False) -> st
 if __name__ == "__main__":
     print(build(force=True, verbose=True))
     print(build(force=True, audit=True))
+    print(build_calls(force=True))

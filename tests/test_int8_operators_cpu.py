@@ -188,6 +188,26 @@ def test_rows_without_a_place_have_none(place):
             assert b in (0, 1) and page in (-1, 5, 6, 7, 99)
 
 
+def test_calls_refuse_what_is_not_on_a_gpu():
+    """The native checks (csrc/calls.cpp) on host tensors, and arguments that are no tensors at all."""
+    from megaattention_b200._native import calls
+    from megaattention_b200.runtime import dequantize_int8, linear_int8, rmsnorm_int8, rope_append
+    x, w = torch.ones(4, 64, dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16)
+    q, s = torch.ones(4, 64, dtype=torch.int8), torch.ones(4)
+    i = torch.ones(2, dtype=torch.int32)
+    h = torch.ones(1, 2, 128, dtype=torch.bfloat16)
+    for bad in (lambda: rmsnorm_int8(x, w), lambda: rmsnorm_int8([1.0], w), lambda: rmsnorm_int8(x, None),
+                lambda: linear_int8(q, s, q, s), lambda: linear_int8(None, s, q, s), lambda: dequantize_int8(q, s),
+                lambda: rope_append(h, h, h, h, h, i[None], i, i, inv_freq=s), lambda: rope_append(h, 3, h, h, h, i, i, i)):
+        with pytest.raises(AssertionError):
+            bad()
+    with pytest.raises(TypeError):
+        calls.linear_int8(q, s)
+    with pytest.raises(TypeError):
+        linear_int8(q, s, q)
+    assert calls.torch_version == torch.__version__
+
+
 def test_weights_in_eight_bits():
     g = torch.Generator().manual_seed(5)
     for n, k, dtype in ((7, 100, torch.float32), (16, 64, torch.bfloat16), (3, 1, torch.float32)):
