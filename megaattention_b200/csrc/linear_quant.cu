@@ -745,38 +745,44 @@ int launch_wide(const ma_linear_quant_args* a, const LinearArgs& p, int sms, int
 }
 
 // Which kernel, and in which form, by estimates of its time in nanoseconds (device time of a call in a chain
-// of calls, beside a start and an end that all of them have):
-//   few tokens: rounds of two CTAs per SM (92 % of them: clusters leave some over) times a part's loads; what
-//   the ring holds comes at once, and parts have to be exchanged.  1 x 4096 x 10240: 3 parts 9.0 us, 2 11.0,
-//   4 13.4; 4 x 300 x 20000: 1 part 4.6, 2 7.7; 10 x 16384 x 2304: 6 parts 9.7, 4 10.7, 3 11.4;
-//   many tokens: rounds of a tile per pair of SMs; 4096 x 4096 x 4096: 256 channels 48 us, 128 54, 64 87;
-//   1384 x 4096 x 1280: 14.4, 10.5, 14.9; 777 x 1000 x 1001: 11.7, 7.9, 6.2.
+// of calls, beside a start and an end that all of them have; over 2900 random sizes the choice took 2 % longer
+// than the best form would have on the average):
+//   few tokens: a block of K takes 160 on an SM that has one CTA, parts have to be exchanged, and the tokens of
+//   a tile written; a round beyond the first starts anew.  1 x 4096 x 10240: 3 parts 9.0 us, 2 11.0, 4 (two
+//   rounds) 13.4; 17 x 1402 x 213: 6 parts 3.3, 3 3.7, 1 4.7; 10 x 16384 x 2304: 6 parts 9.7, 4 10.7, 3 11.4;
+//   many tokens: rounds of a tile per pair of SMs; 4096 x 4096 x 4096: 256 channels 47 us, 128 53, 64 87;
+//   1384 x 4096 x 1280: 14.3, 10.3, 14.9; 256 x 128 x 512: 4.5, 3.5, 2.9.
 // Up to 32 tokens the first always, above 512 the second; in between 64 x 4096 x 4096 takes 8.4 by the first
-// and 9.3 by the second, 64 x 512 x 512 4.1 and 3.3, 300 x 16384 x 2304 19.1 and 25.4.
+// and 9.3 by the second, 64 x 512 x 512 4.1 and 3.3, 300 x 16384 x 2304 19.1 and 25.4, 272 x 930 x 24924 39 and 22.
 struct Form {
   long long tiles, time;
   int width, splits;                         // channels of a tile, or parts of K
 };
 Form narrow_form(const LinearArgs& p, int tn, int sms) {
+  constexpr int kParts[5] = {1, 2, 3, 4, kMaxSplits};
+  constexpr int kRoom[5] = {100, 100, 94, 95, 91};      // % of two CTAs per SM: clusters leave some over
   const long long blocks = (p.inner + kSlab - 1) / kSlab;
   const long long tiles = (p.width + 127LL) / 128 * ((p.tokens + tn - 1LL) / tn);
-  const long long room = 2LL * sms * 92 / 100;
   Form best{0, 0, 0, 0};
-  for (int n : {1, 2, 3, 4, kMaxSplits}) {
-    if (n > blocks) break;
-    const long long load = blocks * 340 / n;
-    const long long time = (tiles * n + room - 1) / room * ((load > 2040 ? load : 2040) + (n > 1 ? 600 + 200 * n : 0));
-    if (n == 1 || time < best.time) best = {tiles * n, time, 0, n};
+  long long least = 0;
+  for (int i = 0; i < 5 && kParts[i] <= blocks; ++i) {
+    const long long n = kParts[i], ctas = tiles * n, room = 2LL * sms * kRoom[i] / 100;
+    const long long rounds = (ctas + room - 1) / room, last = ctas - (rounds - 1) * room, part = blocks * 160 / n;
+    const long long time = (rounds - 1) * (2 * part + 4000) + part * ((last + sms - 1) / sms) +
+                           (n > 1 ? 200 + 60 * n : 0) + (tn / 16 - 1) * (333 + 333 / n);
+    if (i == 0 || time < least) least = time;
+    // (of two about equal ones the one with more loads in flight: 1 x 8192 x 8192 4 parts 13.2, 2 14.2)
+    if (i == 0 || time * 100 <= least * 107) best = {ctas, time, 0, static_cast<int>(n)};
   }
   return best;
 }
 Form wide_form(const LinearArgs& p, int sms) {
   const long long blocks = (p.inner + kSlab - 1) / kSlab;
-  constexpr int kRound[3] = {1000, 1800, 2200}, kBlock[3] = {160, 180, 290};
+  constexpr int kEnd[3] = {150, 500, 860}, kRound[3] = {550, 830, 1440}, kBlock[3] = {160, 180, 290};
   Form best{0, 0, 0, 0};
   for (int i = 0; i < 3; ++i) {
     const long long tiles = (p.tokens + 255LL) / 256 * ((p.width + (64LL << i) - 1) / (64LL << i));
-    const long long time = (tiles + sms / 2 - 1) / (sms / 2) * (kRound[i] + blocks * kBlock[i]);
+    const long long time = (tiles + sms / 2 - 1) / (sms / 2) * (kRound[i] + blocks * kBlock[i]) + kEnd[i];
     if (i == 0 || time < best.time) best = {tiles, time, 64 << i, 0};
   }
   return best;
@@ -787,10 +793,12 @@ int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms,
     const Form f = narrow_form(p, tn, sms);
     if (p.tokens <= 32 || f.time <= wide_form(p, sms).time) {
       if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
-      // an SM that has one CTA only gives it all of its shared memory, where its part is long enough to fill it
-      // (48 x 16384 x 2304: 10.9 us for 12.9; 16 x 4096 x 4096, 8 blocks a part: 6.7 for 6.1); clusters of three
-      // and more find no room on some SMs
-      const bool deep = f.tiles <= (f.splits > 2 ? sms * 88 / 100 : sms) && p.inner >= 16 * kSlab * f.splits;
+      // An SM that has one CTA only gives it all of its shared memory, where its part is long enough to fill it
+      // or SMs are left for the kernel behind this one (48 x 16384 x 2304: 10.9 us for 12.9; 1 x 1524 x 376 3.0 for
+      // 3.6; but 16 x 4096 x 4096, 128 CTAs of 8 blocks, 6.7 for 6.1).  Clusters of three and more find no room on
+      // some SMs.
+      const bool deep = f.tiles <= (f.splits > 2 ? sms * 88 / 100 : sms) &&
+                        (f.tiles * 4 <= sms * 3 || p.inner >= 10 * kSlab * f.splits);
       switch (tn) {
         case 16: return deep ? launch_narrow<16, 11>(a, p, f.splits, dev, stream) : launch_narrow<16, 6>(a, p, f.splits, dev, stream);
         case 32: return deep ? launch_narrow<32, 10>(a, p, f.splits, dev, stream) : launch_narrow<32, 5>(a, p, f.splits, dev, stream);
