@@ -276,7 +276,11 @@ PyObject* rope_append(PyObject* const* a) {
   if (PyObject* o = optional(a[9])) {
     out = tensor(o, "out: as q");
     REQUIRE(heads(out, tokens, H, dev), "out: as q");
-    REQUIRE((out.stride(0) >= 128 || tokens <= 1) && (out.stride(1) >= 128 || H == 1), "heads of out overlap");
+    const auto apart = [&](int inner, int outer) {        // one dimension's heads lie within a step of the other
+      const int64_t ni = out.size(inner), no = out.size(outer), si = out.stride(inner), so = out.stride(outer);
+      return (ni <= 1 || si >= 128) && (no <= 1 || so >= (ni <= 1 ? 0 : (ni - 1) * si) + 128);
+    };
+    REQUIRE(tokens == 0 || apart(1, 0) || apart(0, 1), "heads of out overlap");
   } else {
     out = empty({tokens, H, 128}, at::kBFloat16, dev);
   }

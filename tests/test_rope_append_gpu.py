@@ -242,3 +242,20 @@ def test_a_captured_call_follows_the_arrays():
         torch.cuda.synchronize()
         assert _check(c, out, kc, vc, w) == 0
         assert bool((out[active:] == 7).all())
+
+
+def test_an_output_in_another_order_and_one_that_overlaps():
+    """Heads before tokens, and rows with room between them; heads that share memory are refused."""
+    c = _case([3, 2], [5, 140], 4, 2)
+    plain, kc, vc = _run(c)
+    for out in (torch.zeros(4, 5, 128, dtype=torch.bfloat16, device="cuda").transpose(0, 1),
+                torch.zeros(5, 6, 136, dtype=torch.bfloat16, device="cuda")[:, 1:5, 8:]):
+        got, k, v = _run(c, out=out)
+        assert got is out and torch.equal(got, plain) and torch.equal(k, kc) and torch.equal(v, vc)
+    room = torch.zeros(5 * 4 * 128, dtype=torch.bfloat16, device="cuda")
+    for stride in ((128, 128, 1), (384, 128, 1), (512, 64, 1), (128, 512, 1), (0, 128, 1)):
+        with pytest.raises(AssertionError):
+            _run(c, out=room.as_strided((5, 4, 128), stride))
+    one = dict(c, cu=[0, 1, 1], lens=[5, 0], qkv=c["qkv"][:1])              # (a single token: any step between tokens)
+    got, _, _ = _run(one, out=room.as_strided((1, 4, 128), (0, 128, 1)))
+    assert torch.equal(got, _run(one)[0])
