@@ -58,7 +58,7 @@ def build_calls(force: bool = False) -> str:
            "-I" + os.path.join(cuda, "include"), "-I" + os.path.join(at, "include"),
            "-I" + os.path.join(at, "include", "torch", "csrc", "api", "include"), os.path.join(CSRC, "calls.cpp"),
            "-L" + os.path.join(at, "lib"), "-Wl,-rpath," + os.path.join(at, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
-           "-ltorch_python"]
+           "-ltorch_cuda", "-ltorch_python"]
     return _compile(LIB_CALLS, cmd, force)
 
 
