@@ -32,7 +32,14 @@ namespace {
 // What gave up, as in ma_status {code, site, cta, aux}; one per device.
 __device__ uint32_t g_linear_status[4];
 constexpr uint32_t kCodeTimeout = 1;
+// A call waits for its own copies and products only, never for another kernel or GPU: no argument sets this.
+#ifdef MA_AUDIT
+constexpr uint64_t kWaitLimitNs = 200000000ull;
+// {copies of a CTA that gave up that it had not seen land, those of them that it waited for, CTAs that gave up}
+__device__ uint32_t g_linear_audit[3];
+#else
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
+#endif
 
 __device__ __noinline__ void linear_gave_up(uint32_t site, uint32_t aux) {
   if (atomicCAS(&g_linear_status[0], 0u, kCodeTimeout) == 0u) {
@@ -112,6 +119,9 @@ struct LinearArgs {
   void* out;
   long long out_pitch;
   int tokens, inner, width, out_f32;
+#ifdef MA_AUDIT
+  int stall;                                  // block of K at which the issuer waits for what nobody sends (-1: none)
+#endif
 };
 
 constexpr uint64_t kDescK = smem_desc_template(16, 1024);       // K-major, 128-byte swizzle
@@ -144,7 +154,7 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   constexpr uint32_t kCols = TN < 32 ? 32 : TN;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[STAGES], s_empty[STAGES], s_done;
-  __shared__ uint32_t s_tmem;
+  __shared__ uint32_t s_tmem, s_gave_up, s_sent;
   __shared__ float s_xs[TN];
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5;
@@ -154,6 +164,7 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
     mbar_init(done, 1);
+    s_gave_up = 0;
     fence_mbar_init();
     tma_prefetch_desc(&w_map);
     tma_prefetch_desc(&x_map);
@@ -179,22 +190,24 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       int sent = 0;
       for (; sent < count; ++sent) {
         const int s = sent % STAGES;
-        if (sent >= STAGES && !wait_bounded(empty + 8 * s, (sent / STAGES - 1) & 1, 0x10)) break;
+        if (sent >= STAGES && !wait_bounded(empty + 8 * s, (sent / STAGES - 1) & 1, 0x10)) { s_gave_up = 1; break; }
         const uint32_t at = ring + s * S::kStage;
         mbar_expect_tx(full + 8 * s, S::kStage);
         tma_load_2d(at, &w_map, full + 8 * s, (first + sent) * kSlab, n0);
         tma_load_2d(at + kWBytes, &x_map, full + 8 * s, (first + sent) * kSlab, m0);
       }
-      if (sent < count)                       // gave up: no copy may outlive the CTA
-        for (int i = sent > STAGES ? sent - STAGES : 0; i < sent; ++i)
-          wait_bounded(full + 8 * (i % STAGES), (i / STAGES) & 1, 0x11);
+      s_sent = static_cast<uint32_t>(sent);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (elect_one()) {
       for (int i = 0; i < count; ++i) {
         const int s = i % STAGES;
-        if (!wait_bounded(full + 8 * s, (i / STAGES) & 1, 0x12)) break;
+        uint32_t bar = full + 8 * s, parity = (i / STAGES) & 1;
+#ifdef MA_AUDIT
+        if (first + i == p.stall) { bar = done; parity = 0; }
+#endif
+        if (!wait_bounded(bar, parity, 0x12)) { s_gave_up = 1; break; }
         tc_fence_after();
         const uint32_t a = (ring + s * S::kStage) >> 4, b = a + (kWBytes >> 4);
 #pragma unroll
@@ -203,7 +216,7 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
                  i > 0 || k > 0);
         tc_commit(empty + 8 * s);
       }
-      tc_commit(done);                        // (after a wait that gave up too: nothing is in flight then)
+      tc_commit(done);                        // (after a wait that gave up too)
     }
     __syncwarp();
   }
@@ -216,9 +229,28 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     bias[j] = p.bias && n + j < p.width ? __uint_as_float(static_cast<uint32_t>(p.bias[n + j]) << 16) : 0.f;
   }
   for (int c = tid; c < valid; c += 128) s_xs[c] = p.x_scale[m0 + c];
-  wait_bounded(done, 0, 0x13);
+  if (!wait_bounded(done, 0, 0x13)) s_gave_up = 1;
   tc_fence_after();
   __syncthreads();
+  if (s_gave_up) {
+    // Whichever wait it was: no copy may land in what is the sums' from here on, or outlive the CTA.  Where the
+    // issuer gave up the producer has sent on, so every stage's last copy is waited for.
+    if (tid == 0) {
+      const int sent = static_cast<int>(s_sent);
+      for (int i = sent > STAGES ? sent - STAGES : 0; i < sent; ++i) {
+        const bool landed = wait_bounded(full + 8 * (i % STAGES), (i / STAGES) & 1, 0x11);
+#ifdef MA_AUDIT
+        atomicAdd(&g_linear_audit[0], 1u);
+        atomicAdd(&g_linear_audit[1], landed ? 1u : 0u);
+#endif
+        (void)landed;
+      }
+#ifdef MA_AUDIT
+      atomicAdd(&g_linear_audit[2], 1u);
+#endif
+    }
+    __syncthreads();
+  }
 
   // Thread t holds channel t: its sums go to [token][channel] of this CTA's ring.
   {
@@ -302,6 +334,10 @@ cudaError_t allow_smem(K kernel, int bytes, int dev, std::atomic<uint64_t>* done
   if (e == cudaSuccess && dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
+
+#ifdef MA_AUDIT
+int g_linear_stall = -1;
+#endif
 
 // The tensor maps and the launch; an ma_error.
 template <int TN, int STAGES>
@@ -574,14 +610,23 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
       }
       // every load is used, and no arrival on a barrier of this CTA outstanding, before it ends
+      const uint32_t end = s, end_phase = phase;
       for (int i = 0; i < STAGES && ok; ++i) {
         ok = wait_bounded(empty + 8 * s, phase ^ 1u, 0x24);
         if (++s == STAGES) { s = 0; phase ^= 1u; }
       }
-      if (!ok) {                              // gave up: the copies in flight land long before this is over
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 1000000u) {}
-      }
+      // Gave up: no copy may outlive the pair.  Those of both CTAs are counted here, and the other one waits at
+      // the end of the kernel; a stage's last load was in this phase before `end`, in the one before from there on.
+      if (!ok && rank == 0)
+        for (uint32_t i = 0; i < STAGES; ++i) {
+          const bool landed = wait_bounded(full + 8 * i, i < end ? end_phase : end_phase ^ 1u, 0x25);
+#ifdef MA_AUDIT
+          atomicAdd(&g_linear_audit[0], 1u);
+          atomicAdd(&g_linear_audit[1], landed ? 1u : 0u);
+          if (i == 0) atomicAdd(&g_linear_audit[2], 1u);
+#endif
+          (void)landed;
+        }
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -593,7 +638,11 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         ok = wait_bounded(acc_empty + 8 * acc, ((it >> 1) & 1u) ^ 1u, 0x21);
         tc_fence_after();
         for (int k = 0; k < blocks && ok; ++k) {
-          ok = wait_bounded(full + 8 * s, phase, 0x22);
+          uint32_t bar = full + 8 * s, parity = phase;
+#ifdef MA_AUDIT
+          if (it == 0 && k == p.stall) { bar = acc_full; parity = 0; }
+#endif
+          ok = wait_bounded(bar, parity, 0x22);
           if (!ok) break;
           tc_fence_after();
           const uint32_t a = (ring + s * S::kStage) >> 4, b = a + (S::kA >> 4);
@@ -818,6 +867,18 @@ int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms,
 }  // namespace
 }  // namespace ma
 
+#ifdef MA_AUDIT
+// Test build: the following calls' issuers wait for what nobody sends at this block of K (-1: they do not).
+extern "C" void ma_audit_linear_stall(int block) { ma::g_linear_stall = block; }
+// g_linear_audit since the last call, which it clears.
+extern "C" int ma_audit_linear_counts(uint32_t* out) {
+  const uint32_t zero[3] = {0, 0, 0};
+  return cudaMemcpyFromSymbol(out, ma::g_linear_audit, sizeof(zero)) == cudaSuccess &&
+                 cudaMemcpyToSymbol(ma::g_linear_audit, zero, sizeof(zero)) == cudaSuccess
+             ? MA_OK : MA_ERR_CUDA;
+}
+#endif
+
 extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
   if (!a || !a->x || !a->weight || !a->x_scale || !a->weight_scale || !a->out) return MA_ERR_INVALID;
   if (a->tokens < 0 || a->width < 0 || a->inner < 1) return MA_ERR_INVALID;
@@ -840,6 +901,9 @@ extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
   p.out = reinterpret_cast<void*>(a->out);
   p.out_pitch = a->out_pitch;
   p.tokens = a->tokens; p.inner = a->inner; p.width = a->width; p.out_f32 = a->out_f32;
+#ifdef MA_AUDIT
+  p.stall = ma::g_linear_stall;
+#endif
   return ma::linear_dispatch(a, p, sms, dev, stream);
 }
 
