@@ -446,7 +446,8 @@ int ma_rmsnorm_quant(const ma_rmsnorm_quant_args* args, void* stream);
  * rounded once.  x and weight: 16-byte aligned rows, pitches in elements, multiples of 16 and at least
  * `inner`.  out_pitch >= width in elements; out_f32: fp32 output, otherwise bf16.  bias may be 0.
  * tokens or width 0: nothing to do; inner >= 1.  Asynchronous on `stream`; no allocation.
- * A bounded device-side wait that gives up is reported by ma_linear_status.
+ * A bounded device-side wait that gives up is reported by ma_linear_status; outputs that it left without a sum
+ * are NaN.
  */
 typedef struct ma_linear_quant_args {
   uint64_t x;                        /* i8 [tokens, x_pitch]                              */
@@ -463,7 +464,7 @@ int ma_linear_quant(const ma_linear_quant_args* args, void* stream);
 
 /*
  * Waits for `stream` and reports whether an ma_linear_quant call on the current device gave up since the
- * last report (MA_ERR_DEVICE_TIMEOUT, and *out says where); such a call's output is undefined.
+ * last report (MA_ERR_DEVICE_TIMEOUT, and *out says where); what such a call did not compute is NaN.
  */
 int ma_linear_status(void* stream, ma_status* out);
 

@@ -32,6 +32,10 @@ namespace {
 // What gave up, as in ma_status {code, site, cta, aux}; one per device.
 __device__ uint32_t g_linear_status[4];
 constexpr uint32_t kCodeTimeout = 1;
+// What a CTA that gave up passes on instead of its sums: no sum of 131071 products of bytes is that low.  The
+// outputs that depend on it are NaN, as are those of the tiles that a pair which gave up did not get to.
+constexpr int kNoSum = static_cast<int>(0x80000000u);
+constexpr uint32_t kNaN = 0x7fc00000u;
 // A call waits for its own copies and products only, never for another kernel or GPU: no argument sets this.
 #ifdef MA_AUDIT
 constexpr uint64_t kWaitLimitNs = 200000000ull;
@@ -253,7 +257,11 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   }
 
   // Thread t holds channel t: its sums go to [token][channel] of this CTA's ring.
-  {
+  if (s_gave_up) {
+#pragma unroll 1
+    for (int i = 0; i < TN; ++i)
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring + (i * 128 + tid) * 4), "r"(kNoSum) : "memory");
+  } else {
     constexpr int kCol = TN < 32 ? 16 : 32;
     uint32_t r[TN / kCol][kCol];
 #pragma unroll
@@ -287,14 +295,16 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     for (int u = 0; u < 2; ++u) {
       if (c + 4 * u >= t1) break;
       int sum[4] = {0, 0, 0, 0};
+      bool lost = false;
 #pragma unroll
       for (int r = 0; r < kMaxSplits; ++r) {
+        lost |= part[u][r].x == kNoSum;
         sum[0] += part[u][r].x;
         sum[1] += part[u][r].y;
         sum[2] += part[u][r].z;
         sum[3] += part[u][r].w;
       }
-      const float xs = s_xs[c + 4 * u];
+      const float xs = lost ? __uint_as_float(kNaN) : s_xs[c + 4 * u];
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = fmaf(static_cast<float>(sum[j]) * xs, ws[j], bias[j]);
@@ -653,7 +663,7 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
           tc_commit_pair(empty + 8 * s);
           if (++s == STAGES) { s = 0; phase ^= 1u; }
         }
-        tc_commit_pair(acc_full + 8 * acc);
+        if (ok) tc_commit_pair(acc_full + 8 * acc);      // (a tile that is not complete is not passed on)
       }
     }
     __syncwarp();
@@ -684,7 +694,17 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
       }
       named_bar_sync(1, kWideThreads - 128);
       if (ok) ok = wait_bounded(acc_full + 8 * acc, (it >> 1) & 1u, 0x23);
-      if (!ok) continue;
+      if (!ok) {
+        const int n1 = min(n0 + first + BN / 2, p.width);
+        const long long row = static_cast<long long>(row0 + lane) * p.out_pitch;
+        if (lane < rows)
+#pragma unroll 1
+          for (int n = n0 + first; n < n1; ++n) {
+            if (F32) static_cast<uint32_t*>(p.out)[row + n] = kNaN;
+            else static_cast<uint16_t*>(p.out)[row + n] = static_cast<uint16_t>(kNaN >> 16);
+          }
+        continue;
+      }
       tc_fence_after();
       const uint32_t taddr = tmem + acc * BN + first + (static_cast<uint32_t>((w & 3) * 32) << 16);
       uint32_t r[2][32], u[S::kRow / 4];       // (u: a staged row)

@@ -50,7 +50,7 @@ def _run(lib, x, xs, w, ws, out):
     (m, k), n = x.shape, w.shape[0]
     a = _cabi.LinearQuantArgs(x=x.data_ptr(), weight=w.data_ptr(), x_scale=xs.data_ptr(), weight_scale=ws.data_ptr(),
                               bias=0, out=out.data_ptr(), x_pitch=k, weight_pitch=k, out_pitch=n, tokens=m, inner=k,
-                              width=n, out_f32=1)
+                              width=n, out_f32=int(out.dtype == torch.float32))
     assert lib.ma_linear_quant(C.byref(a), torch.cuda.current_stream().cuda_stream) == _cabi.MA_OK
     torch.cuda.synchronize()
 
@@ -78,3 +78,14 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(audit, m, k
     # (as in tests/test_linear_int8_gpu.py: conversion, two products, and the result's rounding)
     assert bool(((out.double() - ref).abs() <= 5 * 2.0 ** -24 * size).all())
     assert _status(audit)[0] == _cabi.MA_OK and _counts(audit) == [0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,n,block", CASES)
+def test_what_was_not_computed_is_nan(audit, m, k, n, block, dtype):
+    """Every tile lacks a block of its sum, or its pair of CTAs gave up before it; nothing behind the output changes."""
+    x, xs, w, ws = _case(m, k, n)
+    buf = torch.full((m + 1, n), 3.0, device="cuda", dtype=dtype)
+    audit.ma_audit_linear_stall(block)
+    _run(audit, x, xs, w, ws, buf[:m])
+    assert bool(buf[:m].isnan().all()) and bool((buf[m] == 3).all())
