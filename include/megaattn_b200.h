@@ -463,8 +463,9 @@ typedef struct ma_linear_quant_args {
 int ma_linear_quant(const ma_linear_quant_args* args, void* stream);
 
 /*
- * Waits for `stream` and reports whether an ma_linear_quant call on the current device gave up since the
- * last report (MA_ERR_DEVICE_TIMEOUT, and *out says where); what such a call did not compute is NaN.
+ * Waits for `stream` and reports whether an ma_linear_quant call on the current device, on any stream, gave up
+ * since the last report (MA_ERR_DEVICE_TIMEOUT, and *out says where the first one did).  A report goes to one
+ * caller, the first that asks; what such a call did not compute is NaN.
  */
 int ma_linear_status(void* stream, ma_status* out);
 

@@ -17,6 +17,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "../../include/megaattn_b200.h"
 #include "launch.cuh"
@@ -29,8 +30,9 @@ int encode_out_2d(CUtensorMap* out, uint64_t base, bool f32, uint64_t cols, uint
 
 namespace {
 
-// What gave up, as in ma_status {code, site, cta, aux}; one per device.
-__device__ uint32_t g_linear_status[4];
+// What gave up first since the last report, in one word that is taken and cleared in one step: code, site and aux of
+// a byte each (of ma_status), and the CTA.  One per device, so a report takes what any stream's calls left.
+__device__ unsigned long long g_linear_status, g_linear_taken;
 constexpr uint32_t kCodeTimeout = 1;
 // What a CTA that gave up passes on instead of its sums: no sum of 131071 products of bytes is that low.  The
 // outputs that depend on it are NaN, as are those of the tiles that a pair which gave up did not get to.
@@ -46,12 +48,10 @@ constexpr uint64_t kWaitLimitNs = 2000000000ull;
 #endif
 
 __device__ __noinline__ void linear_gave_up(uint32_t site, uint32_t aux) {
-  if (atomicCAS(&g_linear_status[0], 0u, kCodeTimeout) == 0u) {
-    g_linear_status[1] = site;
-    g_linear_status[2] = blockIdx.x;
-    g_linear_status[3] = aux;
-  }
+  atomicCAS(&g_linear_status, 0ull,
+            kCodeTimeout | (site & 255u) << 8 | (aux & 255u) << 16 | static_cast<unsigned long long>(blockIdx.x) << 32);
 }
+__global__ void linear_take_status() { g_linear_taken = atomicExch(&g_linear_status, 0ull); }
 
 // Bounded mbarrier wait (false: gave up).
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, uint32_t site) {
@@ -929,16 +929,17 @@ extern "C" int ma_linear_quant(const ma_linear_quant_args* a, void* stream_) {
 
 extern "C" int ma_linear_status(void* stream, ma_status* out) {
   if (!out) return MA_ERR_INVALID;
-  uint32_t h[4] = {0, 0, 0, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cudaMemcpyFromSymbolAsync(h, ma::g_linear_status, sizeof(h), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+  if (cudaStreamSynchronize(s) != cudaSuccess) return MA_ERR_CUDA;
+  static std::mutex one_at_a_time;             // (g_linear_taken is every report's; the long wait is over)
+  const std::lock_guard<std::mutex> lock(one_at_a_time);
+  unsigned long long w = 0;
+  ma::linear_take_status<<<1, 1, 0, s>>>();
+  if (cudaGetLastError() != cudaSuccess ||
+      cudaMemcpyFromSymbolAsync(&w, ma::g_linear_taken, sizeof(w), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
       cudaStreamSynchronize(s) != cudaSuccess)
     return MA_ERR_CUDA;
-  out->code = h[0]; out->site = h[1]; out->cta = h[2]; out->aux = h[3];
-  if (h[0] == 0) return MA_OK;
-  const uint32_t zero[4] = {0, 0, 0, 0};
-  if (cudaMemcpyToSymbolAsync(ma::g_linear_status, zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return MA_ERR_CUDA;
+  out->code = w & 255; out->site = (w >> 8) & 255; out->cta = static_cast<uint32_t>(w >> 32); out->aux = (w >> 16) & 255;
+  if (out->code == 0) return MA_OK;
   return MA_ERR_DEVICE_TIMEOUT;
 }

@@ -52,8 +52,9 @@ def dequantize_int8(q, scale, *, out=None, out_dtype=torch.bfloat16):
 
 
 def check_linear_status(device=None):
-    """Synchronise the device's current stream and raise if a device-side wait of ``linear_int8`` gave
-    up since the last check (what such a call did not compute is NaN)."""
+    """Synchronise the device's current stream and raise if a device-side wait of ``linear_int8`` on that device
+    gave up since the last check, on whichever stream: one check raises, the first (what such a call did not
+    compute is NaN)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     st = _cabi.Status()
     with torch.cuda.device(dev):

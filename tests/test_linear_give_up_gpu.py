@@ -4,6 +4,7 @@ status says where it gave up, once, and the next call is right.
 The audit build's issuers wait, at a given block of K, for a barrier that nobody arrives at (and for 0.2 s
 instead of 2); everything else is as in the product.  Nothing traps."""
 import ctypes as C
+import threading
 
 import pytest
 import torch
@@ -89,3 +90,27 @@ def test_what_was_not_computed_is_nan(audit, m, k, n, block, dtype):
     audit.ma_audit_linear_stall(block)
     _run(audit, x, xs, w, ws, buf[:m])
     assert bool(buf[:m].isnan().all()) and bool((buf[m] == 3).all())
+
+
+def test_one_of_many_who_ask_at_once_gets_the_report(audit):
+    """A single CTA gives up: a single report, to whoever is first."""
+    x, xs, w, ws = _case(3, 128, 100)
+    out = torch.empty(3, 100, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(8)]
+    for _ in range(5):
+        audit.ma_audit_linear_stall(0)
+        _run(audit, x, xs, w, ws, out)
+        audit.ma_audit_linear_stall(-1)
+        start, got = threading.Barrier(len(streams)), []
+
+        def ask(stream):
+            st = _cabi.Status()
+            start.wait()
+            got.append(audit.ma_linear_status(stream.cuda_stream, C.byref(st)))
+
+        threads = [threading.Thread(target=ask, args=(s,)) for s in streams]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert sorted(got) == [_cabi.MA_ERR_DEVICE_TIMEOUT] + [_cabi.MA_OK] * 7
