@@ -1,5 +1,6 @@
 """The operators' native calls (``csrc/calls.cpp``), built for the torch that is installed and bound to the
-library's entry points.  There is no fallback: without the module importing this raises.
+library's entry points: ``calls``, loaded when it is first used, so that what does without it (the fused path)
+can be imported where it cannot be built.  There is no fallback: without the module its use raises ImportError.
 """
 from __future__ import annotations
 
@@ -27,4 +28,8 @@ def _load():
     return _calls
 
 
-calls = _load()
+def __getattr__(name):           # (only until ``calls`` is there)
+    if name != "calls":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()["calls"] = _load()
+    return calls  # noqa: F821

@@ -17,8 +17,7 @@ import ctypes as C
 
 import torch
 
-from .. import _cabi
-from .._native import calls
+from .. import _cabi, _native
 
 
 def quantize_weight_int8(weight):
@@ -40,7 +39,7 @@ def linear_int8(x, x_scale, weight, weight_scale, *, bias=None, out=None, out_dt
     [out]`` fp32, ``bias [out]`` bf16 or none, all on one CUDA device; ``in`` up to 131071.  Returns
     ``[tokens, out]`` in ``out_dtype`` (bf16 or fp32), or fills ``out`` (any row pitch).  Queued on the
     current stream of that device."""
-    return calls.linear_int8(x, x_scale, weight, weight_scale, bias, out, out_dtype)
+    return _native.calls.linear_int8(x, x_scale, weight, weight_scale, bias, out, out_dtype)
 
 
 def dequantize_int8(q, scale, *, out=None, out_dtype=torch.bfloat16):
@@ -48,7 +47,7 @@ def dequantize_int8(q, scale, *, out=None, out_dtype=torch.bfloat16):
     None]``, rounded once to ``out_dtype`` (bf16 or fp32): an 8-bit weight for what reads 16 bits, as
     ``FusedPrefillLayer(ws, dequantize_int8(W_o, W_o_scale).T)``, or an 8-bit activation beside it.  Queued on
     the current stream of the device."""
-    return calls.dequantize_int8(q, scale, out, out_dtype)
+    return _native.calls.dequantize_int8(q, scale, out, out_dtype)
 
 
 def check_linear_status(device=None):

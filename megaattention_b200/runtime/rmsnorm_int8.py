@@ -19,7 +19,7 @@ product loads them by): of a ``hidden`` that is not a multiple of 16 it is a vie
 """
 from __future__ import annotations
 
-from .._native import calls
+from .. import _native
 
 
 def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, inplace: bool = False, out=None, scale=None):
@@ -28,7 +28,7 @@ def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, inplace: bool =
     ``(q [tokens, hidden] int8, scale [tokens] fp32)``, and the new residual stream as a third where there is a
     residual (with ``inplace`` it is updated where it is).  ``out`` and ``scale`` take the results.
     Queued on the current stream of that device."""
-    return calls.rmsnorm_int8(x, weight, eps, residual, inplace, out, scale, None)
+    return _native.calls.rmsnorm_int8(x, weight, eps, residual, inplace, out, scale, None)
 
 
 def residual_rmsnorm_int8(ws, residual, weight, eps: float = 1e-6, *, inplace: bool = False, out=None, scale=None,
@@ -41,4 +41,4 @@ def residual_rmsnorm_int8(ws, residual, weight, eps: float = 1e-6, *, inplace: b
     tiles = (ws.cu_q.data_ptr(), ws.fa_b.data_ptr(), ws.fa_mb.data_ptr(), int(meta.num_row_tiles),
              int(meta.cu_seqlens_q[-1]), ws.hidden, ws.num_out * 128, ws._stream().cuda_stream)
     with ws._on_stream():                  # (the results' memory is the workspace's stream's too)
-        return calls.rmsnorm_int8(ws.csym, weight, eps, residual, inplace, out, scale, tiles)
+        return _native.calls.rmsnorm_int8(ws.csym, weight, eps, residual, inplace, out, scale, tiles)

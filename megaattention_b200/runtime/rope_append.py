@@ -17,7 +17,7 @@ host, so a captured call follows the arrays' contents.
 """
 from __future__ import annotations
 
-from .._native import calls
+from .. import _native
 from .rope import default_inv_freq
 
 
@@ -36,4 +36,4 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens
     ``theta``.  Queued on the current stream of the device."""
     if inv_freq is None:      # (allocated on this stream: reuse after free is stream-ordered)
         inv_freq = default_inv_freq(theta, q.device)
-    return calls.rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, inv_freq, out, dropped)
+    return _native.calls.rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, inv_freq, out, dropped)
