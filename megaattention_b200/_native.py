@@ -5,6 +5,7 @@ can be imported where it cannot be built.  There is no fallback: without the mod
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 
 import torch
@@ -19,10 +20,12 @@ def _load():
         except Exception as exc:  # no compiler on this machine: use what is there, if anything
             if not os.path.exists(_build.LIB_CALLS):
                 raise ImportError(f"{os.path.basename(_build.LIB_CALLS)} is missing and cannot be built: {exc}")
-    from . import _calls
+    spec = importlib.util.spec_from_file_location(f"{__package__}._calls", _build.LIB_CALLS)
+    _calls = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(_calls)
     if _calls.torch_version != torch.__version__:
         raise ImportError(f"{os.path.basename(_build.LIB_CALLS)} was built for torch {_calls.torch_version}, this is "
-                          f"{torch.__version__}: build it again")
+                          f"{torch.__version__}: delete it")
     _calls.bind(*(C.cast(getattr(_cabi.lib, name), C.c_void_p).value for name in (
         "ma_rmsnorm_quant", "ma_linear_quant", "ma_dequant", "ma_rope_append", "ma_strerror")))
     return _calls

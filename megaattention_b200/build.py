@@ -1,7 +1,9 @@
 """Build the sm_100a shared library in-tree with nvcc (no GPU needed to compile)."""
 from __future__ import annotations
 
+import importlib.util
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -20,9 +22,19 @@ SOURCES = ["fused_prefill.cu", "cabi.cu", "noalloc.cu", "residual_rmsnorm.cu", "
 HEADERS = ["ptx.cuh", "kparams.h", "launch.cuh", "paged.cuh", "append_place.h", os.path.join("..", "..", "include", "megaattn_b200.h")]
 
 
+def torch_version() -> str:
+    """Of the torch that is installed, read without importing it."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return "none"
+    with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:
+        return re.search(r"^__version__ = ['\"]([^'\"]+)", f.read(), re.M).group(1)
+
+
 # The operators' calls natively (csrc/calls.cpp): a Python module over torch's tensors, which hands the C ABI's
-# entry points plain pointers.  Host code only.
-LIB_CALLS = os.path.join(HERE, "_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+# entry points plain pointers.  Host code only.  It works with the torch it was built for, whose version is part of
+# the name: behind another torch it is missing, and built again.
+LIB_CALLS = os.path.join(HERE, f"_calls_torch{torch_version()}" + sysconfig.get_config_var("EXT_SUFFIX"))
 CALLS = ["calls.cpp", os.path.join("..", "..", "include", "megaattn_b200.h")]
 
 

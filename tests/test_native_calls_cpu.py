@@ -1,13 +1,17 @@
 """The operators' native module: what does without it is there without it, and what needs it says so."""
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
+
+import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-def _python(code, **env):
-    return subprocess.run([sys.executable, "-c", code], cwd=ROOT, env={**os.environ, **env}, capture_output=True,
+def _python(code, cwd=ROOT, **env):
+    return subprocess.run([sys.executable, "-c", code], cwd=cwd, env={**os.environ, **env}, capture_output=True,
                           text=True, timeout=600)
 
 
@@ -34,8 +38,39 @@ def test_importing_the_runtime_does_not_load_it():
     got = _python('''
 import sys
 import megaattention_b200.runtime
-assert "megaattention_b200._calls" not in sys.modules
 from megaattention_b200 import _native
+assert "calls" not in vars(_native)
 assert _native.calls is _native.calls and "calls" in vars(_native)
 ''')
     assert got.returncode == 0, got.stderr
+
+
+@pytest.mark.parametrize("entry", ["import", "build"])
+def test_a_module_of_another_torch_is_not_used(tmp_path, entry):
+    """What another torch's build left beside the package, newer than every source, is neither loaded nor taken
+    for this one's: the module is built again (by a compiler that hands out the one that is there)."""
+    from megaattention_b200 import build
+    from megaattention_b200._native import calls
+    here = tmp_path / "megaattention_b200"
+    shutil.copytree(os.path.join(ROOT, "megaattention_b200"), here, ignore=shutil.ignore_patterns("_calls*", "__pycache__"))
+    shutil.copytree(os.path.join(ROOT, "include"), tmp_path / "include")
+    shutil.copy(os.path.join(ROOT, "__graft_entry__.py"), tmp_path)
+    for lib in here.glob("*.so"):
+        os.utime(lib)
+    for name in ("_calls", "_calls_torch0.0.0"):
+        (here / (name + sysconfig.get_config_var("EXT_SUFFIX"))).write_bytes(b"of another torch")
+    cxx = tmp_path / "cxx"
+    cxx.write_text(f"""#!/bin/sh
+while [ $# -gt 1 ]; do if [ "$1" = -o ]; then cp {build.LIB_CALLS} "$2"; fi; shift; done
+echo built >> {tmp_path}/log
+""")
+    cxx.chmod(0o755)
+    got = _python("import __graft_entry__ as g; g.build()\n" * (entry == "build") + f"""
+import torch
+from megaattention_b200 import _native, build
+assert build.HERE == {str(here)!r}, build.HERE
+assert _native.calls.torch_version == torch.__version__ == build.torch_version()
+""", cwd=tmp_path, CXX=str(cxx))
+    assert got.returncode == 0, got.stderr
+    assert (tmp_path / "log").read_text() == "built\n"
+    assert calls.torch_version in os.path.basename(build.LIB_CALLS)
