@@ -4,6 +4,7 @@ from __future__ import annotations
 import importlib.util
 import os
 import re
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -60,14 +61,20 @@ def build(force: bool = False, verbose: bool = False, audit: bool = False) -> st
     return _compile(LIB, cmd + [os.path.join(CSRC, f) for f in SOURCES], force, verbose)
 
 
+def _cuda_include() -> str:
+    """Where CUDA's headers are: of CUDA_HOME, or of the nvcc that compiles the kernels."""
+    nvcc = shutil.which(os.environ.get("NVCC", "nvcc"))
+    home = os.environ.get("CUDA_HOME") or (os.path.dirname(os.path.dirname(os.path.realpath(nvcc))) if nvcc else "/usr/local/cuda")
+    return os.path.join(home, "include")
+
+
 def build_calls(force: bool = False) -> str:
     """Compile ``csrc/calls.cpp`` against the torch that is installed."""
     import torch
     at = os.path.dirname(torch.__file__)
-    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f'-DMA_TORCH_VERSION="{torch.__version__}"', "-I" + sysconfig.get_paths()["include"],
-           "-I" + os.path.join(cuda, "include"), "-I" + os.path.join(at, "include"),
+           "-I" + _cuda_include(), "-I" + os.path.join(at, "include"),
            "-I" + os.path.join(at, "include", "torch", "csrc", "api", "include"), os.path.join(CSRC, "calls.cpp"),
            "-L" + os.path.join(at, "lib"), "-Wl,-rpath," + os.path.join(at, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_cuda", "-ltorch_python"]

@@ -74,3 +74,25 @@ assert _native.calls.torch_version == torch.__version__ == build.torch_version()
     assert got.returncode == 0, got.stderr
     assert (tmp_path / "log").read_text() == "built\n"
     assert calls.torch_version in os.path.basename(build.LIB_CALLS)
+
+
+@pytest.mark.parametrize("home", [False, True])
+def test_cuda_headers_are_those_of_the_compiler_on_the_path(tmp_path, home):
+    """As for the kernels: a toolkit anywhere, if its nvcc is on the path, or CUDA_HOME."""
+    (tmp_path / "toolkit" / "bin").mkdir(parents=True)
+    (tmp_path / "toolkit" / "bin" / "nvcc").write_text("#!/bin/sh\n")
+    cxx = tmp_path / "cxx"
+    cxx.write_text(f"#!/bin/sh\necho \"$@\" > {tmp_path}/log\nexit 1\n")
+    for f in (cxx, tmp_path / "toolkit" / "bin" / "nvcc"):
+        f.chmod(0o755)
+    env = dict(CXX=str(cxx), PATH=f"{tmp_path}/toolkit/bin:{os.environ['PATH']}", CUDA_HOME=str(tmp_path / "home") if home else "")
+    got = _python(f"""
+from megaattention_b200 import build
+build.LIB_CALLS = {str(tmp_path / "_calls.so")!r}
+try:
+    build.build_calls()
+except RuntimeError:
+    print("refused")
+""", NVCC="nvcc", **env)
+    assert got.stdout.strip() == "refused", got.stderr
+    assert f"-I{tmp_path}/{'home' if home else 'toolkit'}/include " in (tmp_path / "log").read_text()
