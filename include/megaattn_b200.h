@@ -417,8 +417,9 @@ int ma_step(ma_plan* plan, const ma_step_args* args, void* stream);
  * `hidden` columns:
  *   h = bf16( float(x) + float(residual) )                     (without a residual: h = x)
  *   y = h * rsqrt(mean(h^2) + eps) * weight in fp32,  scale = max|y| / 127,  q = round(y / scale)
- * A row of zeros gets scale 0 and zeros; one whose sum of squares, maximum or scale is not finite gets
- * scale NaN and zeros.  With cu_q, fa_b, fa_mb (all three or none) x is the fused launch's csym as in
+ * A row of zeros, or whose |h * weight| are all below 1.6e-36, gets scale 0 and zeros; one whose sum of squares,
+ * maximum or scale is not finite, or whose mean(h^2) + eps is below 2^-126 (what fp32 squares hold), gets scale
+ * NaN and zeros.  With cu_q, fa_b, fa_mb (all three or none) x is the fused launch's csym as in
  * ma_residual_rmsnorm and `rows` counts row tiles; the other arrays are packed.  Without them x is packed
  * too and `rows` counts rows.  Pitches are in elements: multiples of 8, q's of 16, none below hidden.
  * x, residuals, weight and q are 16-byte aligned; hidden % 8 == 0; hidden <= 16384, rows <= 2^30 and row

@@ -8,11 +8,14 @@
 // maximum, and both - the sum of h^2 and the maximum of |h w| - come from one pass and one exchange
 // between the warps; h w is exact in fp32 (8-bit by 8-bit significands), the sum is fp32.
 // A row of zeros gets scale 0 and zeros; a row whose sum of squares, maximum or scale is not finite gets
-// scale NaN and zeros, so that what is computed from it is NaN too.
+// scale NaN and zeros, so that what is computed from it is NaN too.  So does one whose mean + eps is below 2^-126:
+// its squares have lost their last bits (down to that, n squares are off by 2^-150 each, 2^-24 of the mean).  A
+// row of products below 1.6e-36 counts as zeros, whatever eps.
 //
 // HBM bound: 3 bytes per element, 7 with a residual.  Device time: 13400 x 4096 28 us (5.8 TB/s, 0.90 of the
 // measured copy rate), with a residual 64 us (6.0 TB/s); 22600 x 16384 174 us (6.4 TB/s) and 412 us (6.3 TB/s).
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "../../include/megaattn_b200.h"
@@ -224,10 +227,11 @@ rmsnorm_quant_kernel(const __grid_constant__ NormQuant p) {
         if (kWarps >= 4) top = nq_max(top, b.z, b.w);
       }
     }
-    float scale = top * rsqrtf(ss * inv_n + p.eps) * (1.f / 127.f);
+    const float mean = ss * inv_n + p.eps;
+    const float scale = top * rsqrtf(mean) * (1.f / 127.f);
     // (below 2^-119 the factor would overflow: such a row's values are below every scale in use)
     const bool none = top < 1.6e-36f;
-    const bool bad = !(top < INFINITY) || !(ss < INFINITY) || (!none && !(scale < INFINITY));
+    const bool bad = !(top < INFINITY) || !(ss < INFINITY) || (!none && !(mean >= FLT_MIN && scale < INFINITY));
     const uint64_t f2 = nq_both(none || bad ? 0.f : 127.f / top);
     if (tid == 0) p.scale[tok] = bad ? __int_as_float(0x7fc00000) : none ? 0.f : scale;
     int8_t* qr = at_row(p.q, tok, p.q_pitch) + tid * 8;

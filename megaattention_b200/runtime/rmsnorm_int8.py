@@ -14,7 +14,9 @@ straight from the fused launch's tile-padded output::
 
 ``h = bf16(x + residual)``, ``y = h * rsqrt(mean(h^2) + eps) * weight``, ``scale = max|y| / 127`` per
 token and ``q = round(y / scale)`` with the statistics in fp32.  A row of zeros gets scale 0 and zeros, a
-row that is not finite scale NaN and zeros.  ``q``'s rows start at multiples of 16 bytes (what the matrix
+row that is not finite (or its sum of squares) scale NaN and zeros.  With an ``eps`` of 0, or close to it, so does a
+row whose ``mean(h^2) + eps`` is below 2^-126, where fp32 squares lose their bits; ``h * weight`` below 1.6e-36
+throughout counts as zeros.  ``q``'s rows start at multiples of 16 bytes (what the matrix
 product loads them by): of a ``hidden`` that is not a multiple of 16 it is a view with a longer row pitch.
 """
 from __future__ import annotations

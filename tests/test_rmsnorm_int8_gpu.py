@@ -115,6 +115,30 @@ def test_rows_of_zeros_tiny_rows_and_rows_that_are_not_finite(hidden):
     assert bool(rmsnorm_int8(x, w)[1].isnan().all())
 
 
+@pytest.mark.parametrize("hidden", [64, 1000, 2048, 16384])
+@pytest.mark.parametrize("residual", [False, True])
+def test_rows_whose_squares_fp32_does_not_hold(hidden, residual):
+    """Rows of 2^-k: right down to a mean of 2^-126, where n squares off by 2^-150 at most are 2^-24 of it (the
+    tolerance has that, as a rounding more); NaN below, not a scale from squares of a few bits; right again
+    behind an eps that is larger."""
+    from megaattention_b200.runtime import rmsnorm_int8
+    powers = [0, 50, 60, 62, 64, 65, 66, 68, 70, 73, 80, 100, 110]
+    x, r, w = _inputs(len(powers), hidden)
+    down = torch.tensor([2.0 ** -k for k in powers], device="cuda")[:, None]
+    x = (x.float() * down).bfloat16()                  # (exact)
+    r = (r.float() * down).bfloat16() if residual else None
+    h = x.double() + r.double() if residual else x.double()
+    mean = h.square().mean(-1).cpu()
+    for eps in (0.0, 2.0 ** -140, 2.0 ** -100, 1e-6):
+        got = rmsnorm_int8(x, w, eps, residual=r)
+        q, scale = got[0].cpu(), got[1].cpu()
+        keep = [i for i in range(len(powers)) if float(mean[i]) + eps >= 2.0 ** -125.9]
+        lost = [i for i in range(len(powers)) if float(mean[i]) + eps < 2.0 ** -126.1]
+        assert len(keep) + len(lost) == len(powers) and len(lost) in ((0,) if eps > 2.0 ** -120 else range(7, 11))
+        _check(q[keep], scale[keep], x[keep], w, eps, None if r is None else r[keep], got[2][keep] if residual else None)
+        assert bool(scale[lost].isnan().all()) and not bool(q[lost].any())
+
+
 def test_tiles_of_the_fused_output_in_place():
     """Three ragged sequences in csym; padding rows hold NaN and are not read as tokens."""
     from megaattention_b200.metadata import build_row_desc
