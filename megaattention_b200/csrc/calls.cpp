@@ -8,7 +8,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/Context.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -52,8 +54,13 @@ bool vector_of(const at::Tensor& t, int64_t n, at::ScalarType type, const c10::D
 int64_t pitch_of(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 16 * 16; }
 bool packed_columns(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1; }
 
-// (without the dispatcher, 0.3 us of each: a norm's three outputs 6.3 -> 5.5 us of host time)
+// Without the dispatcher, 0.3 us of each (a norm's three outputs 6.3 -> 5.5 us of host time), unless somebody wants
+// to see it: a dispatch mode, or the filling of fresh memory under deterministic algorithms.
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const c10::Device& dev) {
+  const at::Context& context = at::globalContext();
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+      (context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory()))
+    return at::empty(size, at::TensorOptions().dtype(type).device(dev));
   return at::Tensor(at::detail::empty_cuda(size, type, dev, std::nullopt));
 }
 

@@ -84,3 +84,49 @@ def test_a_whole_layer_step_in_eight_bits(lens_q, lens_k, H, Hkv, hidden):
     assert torch.equal(res.cpu(), h) and bool(((n2.cpu().double() - tt).abs() <= 0.5 + 127 * 2.0 ** -23).all())
     ref, size = linear_int8_oracle(n2.cpu(), s2.cpu(), *(p.cpu() for p in up8))
     assert bool(((up.cpu().double() - ref).abs() <= 2.0 ** -8 * 1.001 * size).all())
+
+
+def _operators():
+    """Each operator, small, as a call without arguments and the number of outputs that it allocates."""
+    from megaattention_b200.runtime import dequantize_int8, linear_int8, rmsnorm_int8, rope_append
+    from megaattention_b200.runtime.rope import default_inv_freq
+    x, w = torch.ones(5, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    q8, s8 = torch.ones(5, 64, dtype=torch.int8, device="cuda"), torch.ones(5, device="cuda")
+    h = torch.ones(5, 2, 128, dtype=torch.bfloat16, device="cuda")
+    pages = torch.zeros(1, 128, 2, 128, dtype=torch.bfloat16, device="cuda")
+    i = [torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([[0]], [3], [0, 3])]
+    freq = default_inv_freq(1e4, "cuda")
+    return [(lambda: rmsnorm_int8(x, w, residual=x), 3), (lambda: linear_int8(q8, s8, q8, s8), 1),
+            (lambda: dequantize_int8(q8, s8), 1), (lambda: rope_append(h, h, h, pages, pages, *i, inv_freq=freq), 1)]
+
+
+def test_a_dispatch_mode_sees_the_outputs():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    for call, outputs in _operators():
+        want, names = call(), []
+        with Seen():
+            got = call()
+        assert sum("aten.empty" in n for n in names) == outputs, names
+        for a, b in zip(want if outputs > 1 else [want], got if outputs > 1 else [got]):
+            assert torch.equal(a[:3], b[:3])             # (the append's last rows are behind its sequence)
+
+
+def test_fresh_outputs_are_filled_where_torch_fills_them():
+    """Rows that the append does not write: NaN under deterministic algorithms, not what the memory held."""
+    call = _operators()[-1][0]
+    torch.use_deterministic_algorithms(True)
+    try:
+        for _ in range(3):
+            old = torch.full((5, 2, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+            del old                                      # (its memory is the next of this size)
+            out = call()
+            assert bool(out[3:].isnan().all()) and bool(out[:3].isfinite().all())
+            del out
+    finally:
+        torch.use_deterministic_algorithms(False)
