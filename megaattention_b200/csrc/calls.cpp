@@ -251,6 +251,26 @@ bool heads(const at::Tensor& t, int64_t tokens, int64_t n, const c10::Device& de
          t.stride(2) == 1 && (at_of(t) & 15u) == 0 && (t.stride(0) & 7) == 0 && (t.stride(1) & 7) == 0;
 }
 
+// Whether two tensors of heads may share memory.  What lies between the other's tokens does not if both have the same
+// step from token to token, or else from head to head.
+bool mixed(const at::Tensor& a, const at::Tensor& b) {
+  const auto reach = [](const at::Tensor& t, int first) {
+    int64_t n = 128;
+    for (int d = first; d < 2; ++d) n += (t.size(d) - 1) * t.stride(d);
+    return n;
+  };
+  const auto step_of_both = [&](int d) { return a.size(d) <= 1 ? b.stride(d) : b.size(d) <= 1 || a.stride(d) == b.stride(d) ? a.stride(d) : 0; };
+  const auto apart = [](int64_t from_a_to_b, int64_t step, int64_t na, int64_t nb) {
+    const int64_t at = (from_a_to_b % step + step) % step;
+    return at >= na && at + nb <= step;
+  };
+  const int64_t gap = (static_cast<int64_t>(at_of(b)) - static_cast<int64_t>(at_of(a))) / 2;      // elements
+  if (gap >= reach(a, 0) || -gap >= reach(b, 0)) return false;
+  const int64_t token = step_of_both(0), head = step_of_both(1);
+  if (token && apart(gap, token, reach(a, 1), reach(b, 1))) return false;
+  return !(head && (a.size(0) <= 1 || (token && token % head == 0)) && apart(gap, head, 128, 128));
+}
+
 // (q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, inv_freq, out, dropped)
 PyObject* rope_append(PyObject* const* a) {
   const at::Tensor& q = tensor(a[0], "q: [tokens, heads, 128] bf16");
@@ -290,6 +310,11 @@ PyObject* rope_append(PyObject* const* a) {
       return (ni <= 1 || si >= 128) && (no <= 1 || so >= (ni <= 1 ? 0 : (ni - 1) * si) + 128);
     };
     REQUIRE(tokens == 0 || apart(1, 0) || apart(0, 1), "heads of out overlap");
+    // A warp reads its heads before it writes any of them, and another's at any time.
+    const bool in_place = at_of(out) == at_of(q) && (tokens <= 1 || out.stride(0) == q.stride(0)) &&
+                          (H <= 1 || out.stride(1) == q.stride(1));
+    REQUIRE(tokens == 0 || ((in_place || !mixed(out, q)) && !mixed(out, k) && !mixed(out, v)),
+            "out: q itself, or memory that q, k and v have no part in (between their tokens: with their step)");
   } else {
     out = empty({tokens, H, 128}, at::kBFloat16, dev);
   }

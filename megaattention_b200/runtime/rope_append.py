@@ -27,7 +27,8 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens
     of 16 bytes); ``k_cache, v_cache`` bf16, contiguous, ``[num_pages, 128, H_kv, 128]`` or token pools
     ``[num_pages * 128, H_kv, 128]``; ``page_table [batch, pages]``, ``cache_seqlens [batch]`` and
     ``cu_seqlens_q [batch + 1]`` (ascending from 0; sequences may be empty) int32; all on one CUDA device.  Returns
-    the rotated q, contiguous, or in ``out`` (which may be ``q`` itself).
+    the rotated q, contiguous, or in ``out``: ``q`` itself, or memory that is no part of q, k and v (where it lies
+    between their tokens, its own are as far apart as theirs).
 
     Rows from ``cu_seqlens_q[-1]`` on are left as they are (in a new output: undefined).  A row whose
     page is not in the table or not in the cache is not appended; one that would lie before its

@@ -259,3 +259,48 @@ def test_an_output_in_another_order_and_one_that_overlaps():
     one = dict(c, cu=[0, 1, 1], lens=[5, 0], qkv=c["qkv"][:1])              # (a single token: any step between tokens)
     got, _, _ = _run(one, out=room.as_strided((1, 4, 128), (0, 128, 1)))
     assert torch.equal(got, _run(one)[0])
+
+
+def test_an_output_that_shares_memory_with_the_inputs():
+    """Another token's or head's memory is refused (it would be read before or after it is written); q itself and
+    what lies between the inputs' tokens or heads is not."""
+    c = _case([3, 60], [5, 140], 4, 2)
+    want, kc, vc = _run(c)
+    t, n = 63, (4 + 2 * 2) * 128
+    i32 = dict(dtype=torch.int32, device="cuda")
+    index = [torch.tensor(c[x], **i32) for x in ("table", "lens", "cu")]
+
+    def run(q, k, v, out):
+        from megaattention_b200.runtime import rope_append
+        k2, v2 = c["k_cache"].cuda(), c["v_cache"].cuda()
+        return rope_append(q, k, v, k2, v2, *index, out=out), k2, v2
+
+    room = torch.zeros(3 * t * n, dtype=torch.bfloat16, device="cuda")
+    qkv = room[t * n:2 * t * n].view(t, n)
+    qkv.copy_(c["qkv"])
+    q, k, v = _split(qkv, 4, 2)
+    before = room.clone()
+    for shift, stride in ((0, (512, 128)), (n, (n, 128)), (-n, (n, 128)), (8, (n, 128)), (-128, (n, 128)), (128, (n, 128)),
+                          (512, (n, 128)), (768, (n, 128)), (0, (n, 256)), (0, (128, t * 128)), (t * n - 128, (512, 128)),
+                          (-512 * t + 128, (512, 128)), (-512, (n, 128))):
+        with pytest.raises(AssertionError):
+            run(q, k, v, room.as_strided((t, 4, 128), (*stride, 1), t * n + shift))
+    assert torch.equal(room, before)
+    # a place of its own between the tokens, before q and behind v; between the heads; behind everything
+    wide = torch.zeros(t, n + 1024 + 8, dtype=torch.bfloat16, device="cuda")
+    wide[:, 512:512 + n] = qkv
+    pairs = torch.zeros(t, 4, 2, 128, dtype=torch.bfloat16, device="cuda")
+    pairs[:, :, 0] = q
+    packed = (q.contiguous(), k.contiguous(), v.contiguous())
+    for ins, out in ((_split(wide[:, 512:512 + n], 4, 2), wide[:, :512].unflatten(1, (4, 128))),
+                     (_split(wide[:, 512:512 + n], 4, 2), wide[:, 512 + n:1024 + n].unflatten(1, (4, 128))),
+                     ((pairs[:, :, 0], k, v), pairs[:, :, 1]), (packed, pairs[:, :, 1]),
+                     ((q, k, v), room[2 * t * n:][:512 * t].view(t, 4, 128)), ((q, k, v), q)):
+        got, k2, v2 = run(*ins, out)
+        assert got is out and torch.equal(got, want) and torch.equal(k2, kc) and torch.equal(v2, vc)
+    one = [x[:1] for x in _split(c["qkv"].cuda(), 4, 2)]
+    index = [torch.tensor(x, **i32) for x in (c["table"], [5, 0], [0, 1, 1])]
+    with pytest.raises(AssertionError):                  # a single token: k's heads are k's all the same
+        run(*one, one[0].as_strided((1, 4, 128), (8, 128, 1), 128))
+    first = run(*one, None)[0]
+    assert torch.equal(run(*one, one[0].as_strided((1, 4, 128), (8, 128, 1)))[0], first)
