@@ -20,7 +20,8 @@ LIB_AUDIT = os.path.join(HERE, "libmegaattn_b200_audit.so")
 SOURCES = ["fused_prefill.cu", "cabi.cu", "noalloc.cu", "residual_rmsnorm.cu", "rope.cu",
            "detile.cu", "meta_upload.cu", "step.cu", "meta.cpp", "rmsnorm_quant.cu", "linear_quant.cu", "rope_append.cu",
            "dequant.cu"]
-HEADERS = ["ptx.cuh", "kparams.h", "launch.cuh", "paged.cuh", "append_place.h", os.path.join("..", "..", "include", "megaattn_b200.h")]
+HEADERS = ["ptx.cuh", "kparams.h", "launch.cuh", "paged.cuh", "append_place.h", "linear_form.h",
+           os.path.join("..", "..", "include", "megaattn_b200.h")]
 
 
 def torch_version() -> str:

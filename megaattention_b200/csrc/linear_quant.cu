@@ -5,7 +5,7 @@
 //
 // With few tokens the weights' way from memory bounds it (one byte per weight), with many the tensor cores
 // (8192 products per cycle and SM) and, in a long run, the power limit.  Two kernels, each in a few widths;
-// linear_dispatch at the end says which and why.  Device time in a chain of calls, inputs from memory:
+// linear_form.h says which and why.  Device time in a chain of calls, inputs from memory:
 //   tokens x inner x width       time      of the measured copy rate / of twice the measured bf16 rate
 //       1 x  4096 x 10240      8.9 us      0.73 of the copy rate
 //      48 x 16384 x  2304     10.8 us      0.56
@@ -21,6 +21,7 @@
 
 #include "../../include/megaattn_b200.h"
 #include "launch.cuh"
+#include "linear_form.h"
 #include "ptx.cuh"
 
 namespace ma {
@@ -129,7 +130,7 @@ struct LinearArgs {
 };
 
 constexpr uint64_t kDescK = smem_desc_template(16, 1024);       // K-major, 128-byte swizzle
-constexpr int kSlab = 128;                                      // bytes of K per stage
+constexpr int kSlab = kLinearSlab;
 constexpr int kWBytes = 128 * kSlab;
 
 // ------------------------------------------------------------------ few tokens
@@ -138,7 +139,6 @@ constexpr int kWBytes = 128 * kSlab;
 // take a share of K each, and add their sums through each other's shared memory: integers, so the
 // order does not show.  Every CTA has 64 to 180 KB on their way; what is left beside the loads is the start
 // of a kernel and of its first load, the exchange, and the end (1 x 512 x 512 takes 2.7 us).
-constexpr int kMaxSplits = 6;                // parts of K, the CTAs of a cluster
 __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
 
@@ -813,70 +813,19 @@ int launch_wide(const ma_linear_quant_args* a, const LinearArgs& p, int sms, int
   return e == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
-// Which kernel, and in which form, by estimates of its time in nanoseconds (device time of a call in a chain
-// of calls, beside a start and an end that all of them have; over 2900 random sizes the choice took 2 % longer
-// than the best form would have on the average):
-//   few tokens: a block of K takes 160 on an SM that has one CTA, parts have to be exchanged, and the tokens of
-//   a tile written; a round beyond the first starts anew.  1 x 4096 x 10240: 3 parts 9.0 us, 2 11.0, 4 (two
-//   rounds) 13.4; 17 x 1402 x 213: 6 parts 3.3, 3 3.7, 1 4.7; 10 x 16384 x 2304: 6 parts 9.7, 4 10.7, 3 11.4;
-//   many tokens: rounds of a tile per pair of SMs; 4096 x 4096 x 4096: 256 channels 47 us, 128 53, 64 87;
-//   1384 x 4096 x 1280: 14.3, 10.3, 14.9; 256 x 128 x 512: 4.5, 3.5, 2.9.
-// Up to 32 tokens the first always, above 512 the second; in between 64 x 4096 x 4096 takes 8.4 by the first
-// and 9.3 by the second, 64 x 512 x 512 4.1 and 3.3, 300 x 16384 x 2304 19.1 and 25.4, 272 x 930 x 24924 39 and 22.
-struct Form {
-  long long tiles, time;
-  int width, splits;                         // channels of a tile, or parts of K
-};
-Form narrow_form(const LinearArgs& p, int tn, int sms) {
-  constexpr int kParts[5] = {1, 2, 3, 4, kMaxSplits};
-  constexpr int kRoom[5] = {100, 100, 94, 95, 91};      // % of two CTAs per SM: clusters leave some over
-  const long long blocks = (p.inner + kSlab - 1) / kSlab;
-  const long long tiles = (p.width + 127LL) / 128 * ((p.tokens + tn - 1LL) / tn);
-  Form best{0, 0, 0, 0};
-  long long least = 0;
-  for (int i = 0; i < 5 && kParts[i] <= blocks; ++i) {
-    const long long n = kParts[i], ctas = tiles * n, room = 2LL * sms * kRoom[i] / 100;
-    const long long rounds = (ctas + room - 1) / room, last = ctas - (rounds - 1) * room, part = blocks * 160 / n;
-    const long long time = (rounds - 1) * (2 * part + 4000) + part * ((last + sms - 1) / sms) +
-                           (n > 1 ? 200 + 60 * n : 0) + (tn / 16 - 1) * (333 + 333 / n);
-    if (i == 0 || time < least) least = time;
-    // (of two about equal ones the one with more loads in flight: 1 x 8192 x 8192 4 parts 13.2, 2 14.2)
-    if (i == 0 || time * 100 <= least * 107) best = {ctas, time, 0, static_cast<int>(n)};
-  }
-  return best;
-}
-Form wide_form(const LinearArgs& p, int sms) {
-  const long long blocks = (p.inner + kSlab - 1) / kSlab;
-  constexpr int kEnd[3] = {150, 500, 860}, kRound[3] = {550, 830, 1440}, kBlock[3] = {160, 180, 290};
-  Form best{0, 0, 0, 0};
-  for (int i = 0; i < 3; ++i) {
-    const long long tiles = (p.tokens + 255LL) / 256 * ((p.width + (64LL << i) - 1) / (64LL << i));
-    const long long time = (tiles + sms / 2 - 1) / (sms / 2) * (kRound[i] + blocks * kBlock[i]) + kEnd[i];
-    if (i == 0 || time < best.time) best = {tiles, time, 64 << i, 0};
-  }
-  return best;
-}
 int linear_dispatch(const ma_linear_quant_args* a, const LinearArgs& p, int sms, int dev, cudaStream_t stream) {
-  if (p.tokens <= 512) {
-    const int tn = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : 64;
-    const Form f = narrow_form(p, tn, sms);
-    if (p.tokens <= 32 || f.time <= wide_form(p, sms).time) {
-      if (f.tiles > 0x7fffffffLL) return MA_ERR_CAPACITY;
-      // An SM that has one CTA only gives it all of its shared memory, where its part is long enough to fill it
-      // or SMs are left for the kernel behind this one (48 x 16384 x 2304: 10.9 us for 12.9; 1 x 1524 x 376 3.0 for
-      // 3.6; but 16 x 4096 x 4096, 128 CTAs of 8 blocks, 6.7 for 6.1).  Clusters of three and more find no room on
-      // some SMs.
-      const bool deep = f.tiles <= (f.splits > 2 ? sms * 88 / 100 : sms) &&
-                        (f.tiles * 4 <= sms * 3 || p.inner >= 10 * kSlab * f.splits);
-      switch (tn) {
-        case 16: return deep ? launch_narrow<16, 11>(a, p, f.splits, dev, stream) : launch_narrow<16, 6>(a, p, f.splits, dev, stream);
-        case 32: return deep ? launch_narrow<32, 10>(a, p, f.splits, dev, stream) : launch_narrow<32, 5>(a, p, f.splits, dev, stream);
-        default: return deep ? launch_narrow<64, 8>(a, p, f.splits, dev, stream) : launch_narrow<64, 4>(a, p, f.splits, dev, stream);
-      }
-    }
+  const LinearForm f = linear_form(p.tokens, p.inner, p.width, sms);
+  // (tiles are counted in 32 bits, a round beyond the last)
+  if (f.tiles > (f.splits ? 0x7fffffffLL : 0x7fff0000LL)) return MA_ERR_CAPACITY;
+  switch (f.splits ? f.stages : 0) {
+    case 11: return launch_narrow<16, 11>(a, p, f.splits, dev, stream);
+    case 6: return launch_narrow<16, 6>(a, p, f.splits, dev, stream);
+    case 10: return launch_narrow<32, 10>(a, p, f.splits, dev, stream);
+    case 5: return launch_narrow<32, 5>(a, p, f.splits, dev, stream);
+    case 8: return launch_narrow<64, 8>(a, p, f.splits, dev, stream);
+    case 4: return launch_narrow<64, 4>(a, p, f.splits, dev, stream);
+    default: break;
   }
-  const Form f = wide_form(p, sms);
-  if (f.tiles > 0x7fff0000LL) return MA_ERR_CAPACITY;      // (tiles are counted in 32 bits, a round beyond the last)
   switch (f.width) {
     case 64: return launch_wide<64, 9>(a, p, sms, dev, stream);
     case 128: return launch_wide<128, 7>(a, p, sms, dev, stream);
