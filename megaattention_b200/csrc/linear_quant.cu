@@ -69,6 +69,20 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, uint
   return true;
 }
 
+// For a CTA that gave up: the last copy into each of `stages` stages, the first `turn` of which are a lap ahead of the
+// others (`parity` is theirs).
+__device__ __noinline__ void wait_for_copies(uint32_t full, int stages, int turn, uint32_t parity, uint32_t site) {
+  for (int i = 0; i < stages; ++i) {
+    const bool landed = wait_bounded(full + 8 * i, i < turn ? parity : parity ^ 1u, site);
+#ifdef MA_AUDIT
+    atomicAdd(&g_linear_audit[0], 1u);
+    atomicAdd(&g_linear_audit[1], landed ? 1u : 0u);
+    if (i == 0) atomicAdd(&g_linear_audit[2], 1u);
+#endif
+    (void)landed;
+  }
+}
+
 // D[tmem, s32] (+)= A[smem desc, s8] * B[smem desc, s8]
 __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                        uint32_t accumulate) {
@@ -239,20 +253,7 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   if (s_gave_up) {
     // Whichever wait it was: no copy may land in what is the sums' from here on, or outlive the CTA.  Where the
     // issuer gave up the producer has sent on, so every stage's last copy is waited for.
-    if (tid == 0) {
-      const int sent = static_cast<int>(s_sent);
-      for (int i = sent > STAGES ? sent - STAGES : 0; i < sent; ++i) {
-        const bool landed = wait_bounded(full + 8 * (i % STAGES), (i / STAGES) & 1, 0x11);
-#ifdef MA_AUDIT
-        atomicAdd(&g_linear_audit[0], 1u);
-        atomicAdd(&g_linear_audit[1], landed ? 1u : 0u);
-#endif
-        (void)landed;
-      }
-#ifdef MA_AUDIT
-      atomicAdd(&g_linear_audit[2], 1u);
-#endif
-    }
+    if (tid == 0) wait_for_copies(full, STAGES, static_cast<int>(s_sent % STAGES), s_sent / STAGES & 1u, 0x11);
     __syncthreads();
   }
 
@@ -444,6 +445,13 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   return d;
 }
 
+__device__ __noinline__ void fill_nan(void* out, bool f32, long long row, int n, int end) {
+  for (; n < end; ++n) {
+    if (f32) static_cast<uint32_t*>(out)[row + n] = kNaN;
+    else static_cast<uint16_t*>(out)[row + n] = static_cast<uint16_t>(kNaN >> 16);
+  }
+}
+
 struct WideTiles {
   int m, n, total, stored;                   // stored: the output takes TMA stores (16-byte rows)
 };
@@ -627,16 +635,7 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
       }
       // Gave up: no copy may outlive the pair.  Those of both CTAs are counted here, and the other one waits at
       // the end of the kernel; a stage's last load was in this phase before `end`, in the one before from there on.
-      if (!ok && rank == 0)
-        for (uint32_t i = 0; i < STAGES; ++i) {
-          const bool landed = wait_bounded(full + 8 * i, i < end ? end_phase : end_phase ^ 1u, 0x25);
-#ifdef MA_AUDIT
-          atomicAdd(&g_linear_audit[0], 1u);
-          atomicAdd(&g_linear_audit[1], landed ? 1u : 0u);
-          if (i == 0) atomicAdd(&g_linear_audit[2], 1u);
-#endif
-          (void)landed;
-        }
+      if (!ok && rank == 0) wait_for_copies(full, STAGES, static_cast<int>(end), end_phase, 0x25);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -695,14 +694,7 @@ linear_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
       named_bar_sync(1, kWideThreads - 128);
       if (ok) ok = wait_bounded(acc_full + 8 * acc, (it >> 1) & 1u, 0x23);
       if (!ok) {
-        const int n1 = min(n0 + first + BN / 2, p.width);
-        const long long row = static_cast<long long>(row0 + lane) * p.out_pitch;
-        if (lane < rows)
-#pragma unroll 1
-          for (int n = n0 + first; n < n1; ++n) {
-            if (F32) static_cast<uint32_t*>(p.out)[row + n] = kNaN;
-            else static_cast<uint16_t*>(p.out)[row + n] = static_cast<uint16_t>(kNaN >> 16);
-          }
+        if (lane < rows) fill_nan(p.out, F32, static_cast<long long>(row0 + lane) * p.out_pitch, n0 + first, min(n0 + first + BN / 2, p.width));
         continue;
       }
       tc_fence_after();

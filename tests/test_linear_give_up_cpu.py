@@ -56,12 +56,22 @@ def test_the_kernel_keeps_to_the_rule():
     text = open(SRC).read()
     body = text[text.index("linear_narrow_kernel(const"):text.index("allow_smem(K kernel")]
     waits = re.findall(r"wait_bounded\([^;]*?(0x1\d)\)", body)
-    assert sorted(waits) == ["0x10", "0x11", "0x12", "0x13"]
-    for site in ("0x10", "0x12", "0x13"):                            # each of the others is known to all
+    assert sorted(waits) == ["0x10", "0x12", "0x13"]
+    for site in waits:                                               # each of them is known to all
         assert re.search(r"!wait_bounded\([^;]*%s\)\) (\{ )?s_gave_up = 1;" % site, body), site
-    behind = body[body.index("0x13"):]
     assert re.search(r"s_sent = static_cast<uint32_t>\(sent\);", body[:body.index("0x12")])
-    # they meet, then whoever gave up the copies of every stage in use are waited for, and they meet again
-    assert re.search(r"__syncthreads\(\);\s+if \(s_gave_up\) \{.*?for \(int i = sent > STAGES \? sent - STAGES : 0; i < sent;"
-                     r".*?0x11.*?__syncthreads\(\);\s+\}\s+// Thread t holds", re.sub(r"#ifdef MA_AUDIT.*?#endif", "", behind, flags=re.S),
-                     flags=re.S)
+    # they meet, then whoever gave up each stage's last copy is waited for, and they meet again
+    assert re.search(r"0x13.*?__syncthreads\(\);\s+if \(s_gave_up\) \{[^}]*?if \(tid == 0\) wait_for_copies\(full, STAGES, "
+                     r"static_cast<int>\(s_sent % STAGES\), s_sent / STAGES & 1u, 0x11\);\s+__syncthreads\(\);\s+\}",
+                     body, flags=re.S)
+
+
+@pytest.mark.parametrize("stages", [1, 2, 4, 5, 11])
+def test_the_last_copy_into_each_stage_is_the_one_waited_for(stages):
+    """wait_for_copies' parities: of stage i the lap of its last copy, and for a stage without one the parity that
+    reads as over on a fresh barrier."""
+    for sent in range(5 * stages):
+        turn, parity = sent % stages, sent // stages & 1
+        for i in range(stages):
+            laps = [c // stages for c in range(sent) if c % stages == i]
+            assert (parity if i < turn else parity ^ 1) == (laps[-1] & 1 if laps else 1)
