@@ -18,6 +18,13 @@ MA_HD void search_take(int hits, int* lo, int* n) {
   *n = step < rest ? step : rest;
 }
 
+// A batch that fits a warp: lane i has the start of sequence i, lanes from the last one on where that ends (so that
+// lane b + 1 has the end of sequence b), and its number of keys.  Of the sequences `hits` start at or before the row.
+constexpr int kSmallBatch = 31;
+MA_HD int small_start(int lane, int num_batch) { return lane < num_batch ? lane : num_batch; }
+MA_HD int small_keys(int lane, int num_batch) { return lane < num_batch ? lane : num_batch - 1; }
+MA_HD int small_take(int hits) { return (hits > 1 ? hits : 1) - 1; }
+
 // Row t of the sequence [q0, q1) with `len` keys, the new ones counted: its position, and -1 for a row
 // that is not one of the sequence's or lies before its first key.
 MA_HD int position_of(int t, int q0, int q1, int len) {

@@ -65,9 +65,9 @@ struct Place {
 __device__ __forceinline__ Place place_of(const RopeAppend& p, const int* cu_q, int t, int lane) {
   Place at;
   int b = 0, q0, q1, len;
-  if (p.num_batch < 32) {
-    const int start = cu_q[min(lane, p.num_batch)], n = p.lens[min(lane, p.num_batch - 1)];
-    b = max(__popc(__ballot_sync(0xffffffffu, lane < p.num_batch && start <= t)), 1) - 1;
+  if (p.num_batch <= kSmallBatch) {
+    const int start = cu_q[small_start(lane, p.num_batch)], n = p.lens[small_keys(lane, p.num_batch)];
+    b = small_take(__popc(__ballot_sync(0xffffffffu, lane < p.num_batch && start <= t)));
     q0 = __shfl_sync(0xffffffffu, start, b);
     q1 = __shfl_sync(0xffffffffu, start, b + 1);
     len = __shfl_sync(0xffffffffu, n, b);

@@ -237,3 +237,49 @@ def test_oracles_agree_with_other_statements_of_the_same():
     assert dropped == 0 and torch.allclose(out, qo.double(), rtol=2.0 ** -7, atol=1e-5)
     assert torch.allclose(torch.cat([kc[2, :2], kc[0, :4]]), ko.double(), rtol=2.0 ** -7, atol=1e-5)
     assert torch.equal(torch.cat([vc[2, :2], vc[0, :4]]), k) and not bool(vc[1].any())
+
+
+def test_every_row_of_a_batch_that_fits_a_warp_finds_its_sequence(tmp_path):
+    """The kernel's other way to a row's sequence (csrc/append_place.h): 32 lanes' loads one after the other, every
+    index checked, and the two shuffles from the lanes that they name."""
+    cxx = shutil.which("g++")
+    assert cxx, "a C++ compiler is part of the build environment"
+    (tmp_path / "small.cpp").write_text('''
+#include "%s"
+extern "C" int most() { return ma::kSmallBatch; }
+extern "C" int small(const int* cu_q, int num_batch, int t, const int* lens, int* got) {
+  int start[32], keys[32], hits = 0;
+  for (int lane = 0; lane < 32; ++lane) {
+    const int i = ma::small_start(lane, num_batch), j = ma::small_keys(lane, num_batch);
+    if (i < 0 || i > num_batch || j < 0 || j >= num_batch) return -100;
+    start[lane] = cu_q[i];
+    keys[lane] = lens[j];
+    hits += lane < num_batch && start[lane] <= t;
+  }
+  const int b = ma::small_take(hits);
+  if (b < 0 || b + 1 > 31) return -101;
+  got[0] = start[b]; got[1] = start[b + 1]; got[2] = keys[b];
+  return b;
+}
+''' % os.path.join(ROOT, "megaattention_b200", "csrc", "append_place.h"))
+    subprocess.run([cxx, "-std=c++17", "-O1", "-shared", "-fPIC", "-o", str(tmp_path / "small.so"),
+                    str(tmp_path / "small.cpp")], check=True, capture_output=True)
+    lib = C.CDLL(str(tmp_path / "small.so"))
+    assert lib.most() == 31                  # (lane b + 1 is there for the last of them)
+    rng = random.Random(7)
+    for _ in range(300):
+        nb = rng.choice([1, 2, 5, 30, 31])
+        empty = rng.choice([0.0, 0.5, 0.95])
+        lens_q = [0 if rng.random() < empty else rng.randint(1, 5) for _ in range(nb)]
+        lens = (C.c_int * nb)(*[rng.randint(0, 900) for _ in range(nb)])
+        cu = [0]
+        for n in lens_q:
+            cu.append(cu[-1] + n)
+        owner = [b for b, n in enumerate(lens_q) for _ in range(n)]
+        for t in range(cu[-1]):
+            got = (C.c_int * 3)()
+            b = lib.small((C.c_int * (nb + 1))(*cu), nb, t, lens, got)
+            assert b == owner[t] and list(got) == [cu[b], cu[b + 1], lens[b]]
+    for bad in ([0, -7, 8], [0, 2 ** 31 - 1, 8], [-2 ** 31, 4, 8], [8, 4, 0], [2, 4, 8]):     # no wild index
+        for t in (0, 3, 7):
+            assert lib.small((C.c_int * 3)(*bad), 2, t, (C.c_int * 2)(4, 4), (C.c_int * 3)()) in (0, 1)

@@ -304,3 +304,16 @@ def test_an_output_that_shares_memory_with_the_inputs():
         run(*one, one[0].as_strided((1, 4, 128), (8, 128, 1), 128))
     first = run(*one, None)[0]
     assert torch.equal(run(*one, one[0].as_strided((1, 4, 128), (8, 128, 1)))[0], first)
+
+
+@pytest.mark.parametrize("batch", [2, 30, 31, 32, 33, 64])
+@pytest.mark.parametrize("empty", [(), (0,), (-1,), (0, 1, -2, -1), "odd", "even"])
+def test_batches_around_a_warp_with_empty_sequences(batch, empty):
+    """Up to 31 sequences are looked through at once, more in rounds; the first and the last of them empty or not."""
+    gone = {b for b in range(batch) if b % 2 == (empty == "odd")} if isinstance(empty, str) else {e % batch for e in empty}
+    lens_q = [0 if b in gone else 1 + b % 3 for b in range(batch)]
+    c = _case(lens_q, [n + 100 + 9 * b for b, n in enumerate(lens_q)], 4, 2)
+    if not sum(lens_q):
+        assert _run(c)[0].shape[0] == 0
+        return
+    assert _check(c, *_run(c)) == 0
