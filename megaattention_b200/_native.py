@@ -31,8 +31,9 @@ def _load():
     return _calls
 
 
-def __getattr__(name):           # (only until ``calls`` is there)
+def __getattr__(name):
     if name != "calls":
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
-    globals()["calls"] = _load()
-    return calls  # noqa: F821
+    module = globals()["calls"] = _load()
+    globals().pop("__getattr__", None)         # (a look-up in a module that has one takes four times as long)
+    return module
