@@ -56,11 +56,13 @@ bool packed_columns(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) 
 
 // Without the dispatcher, 0.3 us of each (a norm's three outputs 6.3 -> 5.5 us of host time), unless somebody wants
 // to see it: a dispatch mode, or the filling of fresh memory under deterministic algorithms.
-at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const c10::Device& dev) {
+bool outputs_watched() {
   const at::Context& context = at::globalContext();
-  if (c10::impl::TorchDispatchModeTLS::any_modes_set() ||
-      (context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory()))
-    return at::empty(size, at::TensorOptions().dtype(type).device(dev));
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+         (context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory());
+}
+at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const c10::Device& dev, bool watched) {
+  if (watched) return at::empty(size, at::TensorOptions().dtype(type).device(dev));
   return at::Tensor(at::detail::empty_cuda(size, type, dev, std::nullopt));
 }
 
@@ -93,7 +95,7 @@ at::Tensor output(PyObject* given, PyObject* type, int64_t rows, int64_t n, cons
     REQUIRE(THPDtype_Check(type), "out_dtype: a torch.dtype");
     const at::ScalarType t = reinterpret_cast<THPDtype*>(type)->scalar_type;
     REQUIRE(t == at::kBFloat16 || t == at::kFloat, "bf16 or fp32");
-    out = empty({rows, n}, t, dev);
+    out = empty({rows, n}, t, dev, outputs_watched());
     *pitch = n;
   }
   REQUIRE(out.scalar_type() == at::kBFloat16 || out.scalar_type() == at::kFloat, "bf16 or fp32");
@@ -200,6 +202,7 @@ PyObject* rmsnorm_int8(PyObject* const* a) {
   if (inplace < 0) throw Refused{};
   REQUIRE(a[3] != Py_None || !inplace, "inplace needs a residual");
   at::Tensor q, scale, res_out;
+  const bool watched = outputs_watched();
   if (PyObject* o = optional(a[5])) {
     q = tensor(o, "out: [tokens, hidden] int8");
     eight_bit_rows(q, "out: [tokens, hidden] int8 on a CUDA device");
@@ -207,20 +210,20 @@ PyObject* rmsnorm_int8(PyObject* const* a) {
     args.q_pitch = pitch_of(q);
   } else {
     args.q_pitch = (hidden + 15) / 16 * 16;
-    q = empty({tokens, args.q_pitch}, at::kChar, dev);
+    q = empty({tokens, args.q_pitch}, at::kChar, dev, watched);
     if (args.q_pitch != hidden) q = q.narrow(1, 0, hidden);
   }
   if (PyObject* o = optional(a[6])) {
     scale = tensor(o, "scale: [tokens] fp32");
     REQUIRE(vector_of(scale, tokens, at::kFloat, dev), "scale: [tokens] fp32 on the device of x");
   } else {
-    scale = empty({tokens}, at::kFloat, dev);
+    scale = empty({tokens}, at::kFloat, dev, watched);
   }
   if (PyObject* o = optional(a[3])) {
     const at::Tensor& residual = tensor(o, "residual: [tokens, hidden] bf16");
     REQUIRE(bf16_rows(residual, tokens, hidden, dev),
             "residual: [tokens, hidden] bf16 on the device of x, rows must start at multiples of 16 bytes");
-    res_out = inplace ? residual : empty({tokens, hidden}, at::kBFloat16, dev);
+    res_out = inplace ? residual : empty({tokens, hidden}, at::kBFloat16, dev, watched);
     args.residual_in = at_of(residual); args.residual_out = at_of(res_out);
     args.residual_in_pitch = pitch_of(residual);
     args.residual_out_pitch = inplace ? args.residual_in_pitch : hidden;
@@ -316,7 +319,7 @@ PyObject* rope_append(PyObject* const* a) {
     REQUIRE(tokens == 0 || ((in_place || !mixed(out, q)) && !mixed(out, k) && !mixed(out, v)),
             "out: q itself, or memory that q, k and v have no part in (between their tokens: with their step)");
   } else {
-    out = empty({tokens, H, 128}, at::kBFloat16, dev);
+    out = empty({tokens, H, 128}, at::kBFloat16, dev, outputs_watched());
   }
   ma_rope_append_args args{};
   if (PyObject* o = optional(a[10])) {
