@@ -25,12 +25,19 @@ HEADERS = ["ptx.cuh", "kparams.h", "launch.cuh", "paged.cuh", "append_place.h", 
 
 
 def torch_version() -> str:
-    """Of the torch that is installed, read without importing it."""
+    """Of the torch that is installed, read without importing it where it stands in the usual place."""
     spec = importlib.util.find_spec("torch")
     if spec is None:
         return "none"
-    with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:
-        return re.search(r"^__version__ = ['\"]([^'\"]+)", f.read(), re.M).group(1)
+    try:
+        with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:
+            found = re.search(r"^__version__\b[^=\n]*= *['\"]([^'\"]+)", f.read(), re.M)
+    except (OSError, TypeError):
+        found = None
+    if found:
+        return found.group(1)
+    import torch
+    return str(torch.__version__)
 
 
 # The operators' calls natively (csrc/calls.cpp): a Python module over torch's tensors, which hands the C ABI's

@@ -96,3 +96,18 @@ except RuntimeError:
 """, NVCC="nvcc", **env)
     assert got.stdout.strip() == "refused", got.stderr
     assert f"-I{tmp_path}/{'home' if home else 'toolkit'}/include " in (tmp_path / "log").read_text()
+
+
+@pytest.mark.parametrize("version", ["__version__ = '7.1.2+cu999'", '__version__: str = "7.1.2+cu999"', "import os", None])
+def test_the_version_of_torch_is_found_wherever_it_stands(tmp_path, version):
+    """Importing the package does without importing torch only if it can."""
+    (tmp_path / "torch").mkdir()
+    (tmp_path / "torch" / "__init__.py").write_text("__version__ = '7.1.2+cu999'\n")
+    if version is not None:
+        (tmp_path / "torch" / "version.py").write_text(f"from typing import Optional\n{version}\ncuda = '12.8'\n")
+    got = _python("""
+import sys
+from megaattention_b200 import build
+print(build.torch_version(), "_calls_torch7.1.2+cu999." in build.LIB_CALLS, "torch" in sys.modules)
+""", PYTHONPATH=str(tmp_path))
+    assert got.stdout.split() == ["7.1.2+cu999", "True", str(version is None or "version" not in version)], got.stderr
