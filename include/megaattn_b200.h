@@ -423,8 +423,8 @@ int ma_step(ma_plan* plan, const ma_step_args* args, void* stream);
  * ma_residual_rmsnorm and `rows` counts row tiles; the other arrays are packed.  Without them x is packed
  * too and `rows` counts rows.  Pitches are in elements: multiples of 8, q's of 16, none below hidden.
  * x, residuals, weight and q are 16-byte aligned; hidden % 8 == 0; hidden <= 16384, rows <= 2^30 and row
- * tiles <= 2^23 (MA_ERR_CAPACITY beyond).  residual_out may be residual_in; both are 0 without a
- * residual.  Columns between hidden and q_pitch are left as they are.  Asynchronous on `stream`.
+ * tiles <= 2^23 (MA_ERR_CAPACITY beyond).  residual_out may be residual_in (and x); both are 0 without a
+ * residual.  Rows of q may lie in the same rows of packed x; other outputs share no memory with inputs.  Columns between hidden and q_pitch are left as they are.  Asynchronous on `stream`.
  */
 typedef struct ma_rmsnorm_quant_args {
   uint64_t x, residual_in, weight;   /* bf16                                              */
@@ -446,7 +446,8 @@ int ma_rmsnorm_quant(const ma_rmsnorm_quant_args* args, void* stream);
  * The sum is exact (32-bit integers; inner <= 131071, MA_ERR_CAPACITY beyond), the rest is fp32 and
  * rounded once.  x and weight: 16-byte aligned rows, pitches in elements, multiples of 16 and at least
  * `inner`.  out_pitch >= width in elements; out_f32: fp32 output, otherwise bf16.  bias may be 0.
- * tokens or width 0: nothing to do; inner >= 1.  Asynchronous on `stream`; no allocation.
+ * tokens or width 0: nothing to do; inner >= 1.  out shares no memory with an input.  Asynchronous on
+ * `stream`; no allocation.
  * A bounded device-side wait that gives up is reported by ma_linear_status; outputs that it left without a sum
  * are NaN.
  */
@@ -472,7 +473,8 @@ int ma_linear_status(void* stream, ma_status* out);
 
 /*
  * Rows of 8-bit integers as the values they stand for: out[r, c] = q[r, c] * scale[r], rounded once to
- * bf16 (out_f32: fp32).  q: 16-byte aligned rows, pitch a multiple of 16; out: any pitch.  Asynchronous.
+ * bf16 (out_f32: fp32).  q: 16-byte aligned rows, pitch a multiple of 16; out: any pitch, no memory of
+ * q's or scale's.  Asynchronous.
  */
 typedef struct ma_dequant_args {
   uint64_t q, scale, out;            /* i8, f32 [rows], bf16 or f32                       */

@@ -78,6 +78,32 @@ void queue(F fn, const A& args, const c10::Device& dev, void* stream, const char
   report(fn(&args, stream ? stream : static_cast<void*>(c10::cuda::getCurrentCUDAStream(dev.index()).stream())), what);
 }
 
+// Memory that a call reads or writes, as rows of bytes; a vector is one row.
+struct Rows {
+  int64_t at, rows, pitch, bytes;
+};
+Rows rows_of(const at::Tensor& t) {
+  const int64_t item = t.element_size();
+  const bool vector = t.dim() == 1;
+  return {static_cast<int64_t>(at_of(t)), vector ? 1 : t.size(0), vector ? 0 : t.stride(0) * item, t.size(vector ? 0 : 1) * item};
+}
+// Whether no byte is both's.  What lies between the other's rows is not, if both have the same step from row to row.
+bool apart(const Rows& a, const Rows& b) {
+  const int64_t gap = b.at - a.at;
+  if (gap >= (a.rows - 1) * a.pitch + a.bytes || -gap >= (b.rows - 1) * b.pitch + b.bytes) return true;
+  const int64_t step = a.rows <= 1 ? b.pitch : b.rows <= 1 || a.pitch == b.pitch ? a.pitch : 0;
+  if (!step) return false;
+  const int64_t at = (gap % step + step) % step;
+  return at >= a.bytes && at + b.bytes <= step;
+}
+// Whether a row of one shares memory with the same row of the other only.
+bool row_for_row(const Rows& a, const Rows& b) {
+  if (a.rows <= 1) return true;
+  const int64_t gap = b.at - a.at;
+  return a.pitch == b.pitch && (gap >= 0 ? gap + b.bytes : a.bytes - gap) <= a.pitch;
+}
+bool same_place(const Rows& a, const Rows& b) { return a.at == b.at && (a.rows <= 1 || a.pitch == b.pitch); }
+
 PyObject* optional(PyObject* o) { return o == Py_None ? nullptr : o; }
 
 // An output of `rows` x `n` in the asked type, or the caller's: its row pitch, and whether it is fp32.
@@ -133,6 +159,12 @@ PyObject* linear_int8(PyObject* const* a) {
   ma_linear_quant_args args{};
   const at::Tensor out = output(a[5], a[6], tokens, width, dev, &args.out_pitch, &args.out_f32);
   if (tokens && width) {
+    if (optional(a[5])) {
+      const Rows o = rows_of(out);
+      REQUIRE(apart(o, rows_of(x)) && apart(o, rows_of(w)) && apart(o, rows_of(xs)) && apart(o, rows_of(ws)) &&
+                  (!bias || apart(o, {static_cast<int64_t>(bias), 1, 0, 2 * width})),
+              "out shares memory with an input");
+    }
     args.x = at_of(x); args.weight = at_of(w); args.x_scale = at_of(xs); args.weight_scale = at_of(ws);
     args.bias = bias; args.out = at_of(out);
     args.x_pitch = pitch_of(x); args.weight_pitch = pitch_of(w);
@@ -155,6 +187,8 @@ PyObject* dequantize_int8(PyObject* const* a) {
   ma_dequant_args args{};
   const at::Tensor out = output(a[2], a[3], rows, n, dev, &args.out_pitch, &args.out_f32);
   if (rows && n) {
+    REQUIRE(!optional(a[2]) || (apart(rows_of(out), rows_of(q)) && apart(rows_of(out), rows_of(scale))),
+            "out shares memory with an input");
     args.q = at_of(q); args.scale = at_of(scale); args.out = at_of(out);
     args.q_pitch = pitch_of(q);
     args.rows = static_cast<int32_t>(rows); args.cols = static_cast<int32_t>(n);
@@ -229,6 +263,16 @@ PyObject* rmsnorm_int8(PyObject* const* a) {
     args.residual_out_pitch = inplace ? args.residual_in_pitch : hidden;
   }
   if (tokens) {
+    if (optional(a[5]) || optional(a[6]) || inplace) {
+      // A row is read whole before its integers are written, and the residual by the thread that writes it.
+      const bool packed = a[7] == Py_None;
+      const Rows xr = packed ? rows_of(x) : Rows{static_cast<int64_t>(at_of(x)), 1, 0, x.numel() * 2}, wr = rows_of(w),
+                 qr = rows_of(q), sr = rows_of(scale), rr = args.residual_in ? rows_of(tensor(a[3], "")) : wr;
+      REQUIRE(apart(qr, wr) && apart(sr, wr) && apart(sr, xr) && apart(sr, rr) && apart(sr, qr) &&
+                  (apart(qr, xr) || (packed && row_for_row(qr, xr))) && (apart(qr, rr) || (!inplace && row_for_row(qr, rr))) &&
+                  (!inplace || (apart(rr, wr) && (apart(rr, xr) || (packed && same_place(rr, xr))))),
+              "out, scale or the updated residual shares memory with an input or another of them");
+    }
     args.x = at_of(x); args.weight = at_of(w); args.q_out = at_of(q); args.scale_out = at_of(scale);
     args.rows = static_cast<int32_t>(rows); args.hidden = static_cast<int32_t>(hidden);
     args.eps = static_cast<float>(eps);

@@ -37,8 +37,8 @@ def linear_int8(x, x_scale, weight, weight_scale, *, bias=None, out=None, out_dt
     """``x [tokens, in]`` and ``weight [out, in]`` int8 with rows at multiples of 16 bytes (as
     ``rmsnorm_int8`` and ``quantize_weight_int8`` make them), ``x_scale [tokens]`` and ``weight_scale
     [out]`` fp32, ``bias [out]`` bf16 or none, all on one CUDA device; ``in`` up to 131071.  Returns
-    ``[tokens, out]`` in ``out_dtype`` (bf16 or fp32), or fills ``out`` (any row pitch).  Queued on the
-    current stream of that device."""
+    ``[tokens, out]`` in ``out_dtype`` (bf16 or fp32), or fills ``out`` (any row pitch; no memory of the inputs).
+    Queued on the current stream of that device."""
     return _native.calls.linear_int8(x, x_scale, weight, weight_scale, bias, out, out_dtype)
 
 

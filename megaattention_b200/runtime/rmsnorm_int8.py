@@ -28,7 +28,9 @@ def rmsnorm_int8(x, weight, eps: float = 1e-6, *, residual=None, inplace: bool =
     """``x [tokens, hidden]``, ``weight [hidden]`` and, if given, ``residual [tokens, hidden]`` bf16 on
     one CUDA device; rows at multiples of 16 bytes, ``hidden`` a multiple of 8 up to 16384.  Returns
     ``(q [tokens, hidden] int8, scale [tokens] fp32)``, and the new residual stream as a third where there is a
-    residual (with ``inplace`` it is updated where it is).  ``out`` and ``scale`` take the results.
+    residual (with ``inplace`` it is updated where it is).  ``out`` and ``scale`` take the results; they and an
+    updated residual share no memory with each other or an input, except that ``out``'s rows may lie in ``x``'s (row
+    for row) and that the residual may be ``x``.
     Queued on the current stream of that device."""
     return _native.calls.rmsnorm_int8(x, weight, eps, residual, inplace, out, scale, None)
 

@@ -201,3 +201,35 @@ def test_captured_calls_two_streams_and_equal_bits():
         torch.cuda.synchronize()
         for a, b, c in zip(want, outs, plain):
             assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("m", [5, 700])
+def test_outputs_that_share_memory_with_an_input(m):
+    """Refused, as the inputs are read while outputs are written; columns of one buffer that are the output's alone
+    are not."""
+    from megaattention_b200.runtime import dequantize_int8, linear_int8
+    g = torch.Generator().manual_seed(m)
+    room = torch.zeros(m, 4096, dtype=torch.int8, device="cuda")
+    x = room[:, :1024]
+    x.copy_(_rows(m, 1024, g))
+    w, b = _rows(256, 1024, g), torch.randn(256, generator=g).bfloat16().cuda()
+    xs, ws = torch.rand(m, generator=g).cuda(), torch.rand(256, generator=g).cuda() / 1000
+    wide = room.view(torch.bfloat16)                     # [m, 2048], x in the first 512 of its columns
+    before = room.clone()
+    for out in (wide[:, :256], wide[:, 511:767], wide[:, 256:512], wide.view(-1)[:m * 256].view(m, 256)):
+        with pytest.raises(AssertionError):
+            linear_int8(x, xs, w, ws, bias=b, out=out)
+    square = torch.zeros(256, 256, dtype=torch.bfloat16, device="cuda")
+    scales = square.view(-1).view(torch.float32)[:256]
+    call = dict(x=_rows(256, 256, g), x_scale=ws, weight=_rows(256, 256, g), weight_scale=ws, bias=b)
+    for kw in (dict(bias=square[2]), dict(weight_scale=scales), dict(x_scale=scales),
+               dict(weight=square.view(torch.int8)[:, :256])):
+        with pytest.raises(AssertionError):
+            linear_int8(**{**call, **kw}, out=square)
+    for q, out in ((x, wide[:, :1024]), (room[:, :64], wide[:, 30:94])):
+        with pytest.raises(AssertionError):
+            dequantize_int8(q, xs, out=out)
+    assert torch.equal(room, before)
+    _check(linear_int8(x, xs, w, ws, bias=b, out=wide[:, 512:768]), x, xs, w, ws, b)
+    assert torch.equal(dequantize_int8(x, xs, out=wide[:, 1024:]), (x.float() * xs[:, None]).bfloat16())
+    assert torch.equal(x, before[:, :1024])

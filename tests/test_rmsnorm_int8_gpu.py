@@ -225,3 +225,45 @@ def test_captured_call_and_another_stream():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(rmsnorm_int8(x2, w, residual=r2), out))
+
+
+@pytest.mark.parametrize("tokens,hidden", [(700, 512), (700, 4096), (37, 16384), (1, 1024)])
+def test_outputs_that_share_memory(tokens, hidden):
+    """What another row reads, or two outputs write, is refused; integers in their own row of x, column slices of one
+    buffer and a residual that is x itself are not, and are right."""
+    from megaattention_b200.runtime import rmsnorm_int8
+    x, r, w = _inputs(tokens, hidden)
+    want, want_r = rmsnorm_int8(x, w), rmsnorm_int8(x, w, residual=r)
+
+    def half(t, second=False):                             # of each row's bytes: where its integers find room
+        return t.view(torch.int8)[:, hidden:] if second else t.view(torch.int8)[:, :hidden]
+
+    for second in (False, True):
+        own, other = x.clone(), r.clone()
+        got = rmsnorm_int8(own, w, out=half(own, second))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        got = rmsnorm_int8(x, w, residual=other, out=half(other, second))
+        assert all(torch.equal(a, b) for a, b in zip(got, want_r))
+    both = torch.cat([x, r], 1)
+    got = rmsnorm_int8(both[:, :hidden], w, residual=both[:, hidden:], inplace=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want_r)) and torch.equal(both[:, :hidden], x)
+    twice = x.clone()
+    got = rmsnorm_int8(twice, w, residual=twice, inplace=True)
+    _check(got[0], got[1], x, w, 1e-6, x, got[2])
+
+    room = torch.zeros(tokens + 2, hidden, dtype=torch.bfloat16, device="cuda")
+    mid = room[1:-1]
+    mid.copy_(x)
+    before, floats = room.clone(), room.view(-1).view(torch.float32)
+    eight = torch.zeros(tokens, hidden, dtype=torch.int8, device="cuda")
+    bad = [dict(scale=floats[hidden // 2:][:tokens]), dict(out=half(mid), residual=mid, inplace=True),
+           dict(out=eight, scale=eight.view(-1).view(torch.float32)[:tokens])]
+    if tokens > 1:                                         # other rows' memory
+        bad += [dict(out=mid.view(torch.int8).view(-1)[:tokens * hidden].view(tokens, hidden)), dict(out=half(room[:-2])),
+                dict(out=half(room[2:], True)), dict(residual=room[:-2], inplace=True), dict(residual=room[2:], inplace=True)]
+    for kw in bad:
+        with pytest.raises(AssertionError):
+            rmsnorm_int8(mid, w, **kw)
+    with pytest.raises(AssertionError):
+        rmsnorm_int8(mid[:1], mid[0], out=half(mid[:1]))   # its own weights
+    assert torch.equal(room, before)
