@@ -424,7 +424,8 @@ int ma_step(ma_plan* plan, const ma_step_args* args, void* stream);
  * too and `rows` counts rows.  Pitches are in elements: multiples of 8, q's of 16, none below hidden.
  * x, residuals, weight and q are 16-byte aligned; hidden % 8 == 0; hidden <= 16384, rows <= 2^30 and row
  * tiles <= 2^23 (MA_ERR_CAPACITY beyond).  residual_out may be residual_in (and x); both are 0 without a
- * residual.  Rows of q may lie in the same rows of packed x; other outputs share no memory with inputs.  Columns between hidden and q_pitch are left as they are.  Asynchronous on `stream`.
+ * residual.  Rows of q may lie in the same rows of packed x; other outputs share no memory with inputs.
+ * Columns between hidden and q_pitch are left as they are.  Asynchronous on `stream`.
  */
 typedef struct ma_rmsnorm_quant_args {
   uint64_t x, residual_in, weight;   /* bf16                                              */
