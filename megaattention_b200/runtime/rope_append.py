@@ -33,9 +33,8 @@ def rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens
     Rows from ``cu_seqlens_q[-1]`` on are left as they are (in a new output: undefined).  A row whose
     page is not in the table or not in the cache is not appended; one that would lie before its
     sequence's first key is passed over; ``dropped`` (int32 ``[1]``, on the device) is added the number of
-    both.  Two rows must not have the same place in the cache, nor a
-    row's place be where another's k or v lies.  ``inv_freq [64]`` fp32 takes the place of
-    ``theta``.  Queued on the current stream of the device."""
+    both.  Two rows must not have the same place in the cache, nor a row's place be where another's k or v lies.
+    ``inv_freq [64]`` fp32 takes the place of ``theta``.  Queued on the current stream of the device."""
     if inv_freq is None:      # (allocated on this stream: reuse after free is stream-ordered)
         inv_freq = default_inv_freq(theta, q.device)
     return _native.calls.rope_append(q, k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, inv_freq, out, dropped)
